@@ -533,6 +533,49 @@ int pvx_bn_act_bwd_sync(const void* dy, const void* x, const void* y, int n, int
                         void* stream);
 
 /* ----------------------------------------------------------------------------------------------------
+ * Rows of a table [m, width] looked up by index, and the gradient by sorted index (the counterpart of the scatter ops above: what
+ * broadcasts voxel features back to their points, and what an embedding is).  index: n int32 (index64 == 0) or int64 entries on the
+ * device; entries outside [0, m) give rows of zeros and no gradient.
+ *   pvx_lookup_rows       out[i] = scale table[index[i]] (dtype of the table, rounded once; scale == 1 copies)
+ *   pvx_sort_index        order [n] = the positions by ascending index, equal ones in ascending position, those outside [0, m) at the
+ *                         end; keys [n] = the sorted indices (m for those outside); offsets [m + 1]: row v's run is
+ *                         order[offsets[v]] .. order[offsets[v + 1]].  m >= 1
+ *   pvx_lookup_rows_grad  dtable[v] = scale * sum of dout over row v's run in that order, in binary32, rounded once; rows with no
+ *                         entry are zero, every row is written.  No atomics: the same result on every run.
+ * ---------------------------------------------------------------------------------------------------- */
+int pvx_lookup_rows(const void* table, int dtype, const void* index, int index64, int n, int m, int width, float scale, void* out,
+                    void* stream);
+size_t pvx_sort_index_workspace_bytes(int n);
+int pvx_sort_index(const void* index, int index64, int n, int m, int* order, int* keys, int* offsets, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width);
+int pvx_lookup_rows_grad(const void* dout, int dtype, const int* order, const int* keys, const int* offsets, int n, int m, int width,
+                         float scale, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------------------------
+ * Group norm over the rows of a channels-last matrix x [n, c], fused with (+ residual) -> activation: the normalisation for a
+ * training step whose batches are too small, or too costly to synchronise, for batch statistics.  The rows belong to `samples`
+ * samples: sample s owns the positions offsets[s] .. offsets[s + 1] (device, ascending, samples + 1 entries; NULL: equal samples of
+ * n / samples rows), and position p is row order[p] (device, a permutation of 0 .. n - 1; NULL: row p).  For the rows of a sample and
+ * the c / groups channels of a group, with mean and biased variance over both:
+ *   fwd: z = weight (x - mean) / sqrt(var + eps) + bias (+ residual), y = act(z); save_mean / save_rstd [samples, groups] f32
+ *   bwd: gz = dy act'(z); dbias = sum gz, dweight = sum gz xhat, dresidual = gz,
+ *        dx = (weight gz - mean(weight gz) - xhat mean(weight gz xhat)) / sqrt(var + eps)
+ * Rows at positions of no sample get 0 in y, dx and dresidual; an empty sample gives nothing.  dtype is that of x, residual, y and
+ * their gradients, param_dtype that of weight, bias (NULL: 1 and 0), dweight and dbias (NULL: not wanted).  Deterministic; sums in
+ * binary64.  The gelu is z Phi(z) with the error function.  n == 0 is allowed (dweight = dbias = 0).
+ * ---------------------------------------------------------------------------------------------------- */
+enum { PVX_ACT_NONE = 0, PVX_ACT_RELU = 1, PVX_ACT_SILU = 2, PVX_ACT_GELU = 3 };
+size_t pvx_group_norm_act_workspace_bytes(int n, int c, int samples, int ragged /* offsets given */, int groups);
+int pvx_group_norm_act_fwd(const void* x, int n, int c, int dtype, int samples, const int* offsets, const int* order, int groups,
+                           const void* weight, const void* bias, int param_dtype, float eps, const void* residual, int act,
+                           void* y, float* save_mean, float* save_rstd, void* workspace, size_t workspace_bytes, void* stream);
+int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, int n, int c, int dtype, int samples,
+                           const int* offsets, const int* order, int groups, const void* weight, const void* bias,
+                           int param_dtype, const float* save_mean, const float* save_rstd, int act, void* dx, void* dresidual,
+                           void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------------------------
  * Point-level preparation ahead of the voxelizer: the world augmentations and the range mask /
  * shuffle the reference runs with numpy in DataLoader workers.  binary32 arithmetic in the reference's order (numpy 1.x casting:
  * the drawn float64 scalars act as float32), no contraction.

@@ -24,7 +24,12 @@ from .spconv import pytorch as spconv
 BN_EPS, BN_MOMENTUM = 1e-3, 0.01     # spconv_backbone.py:75,192
 
 
-def _norm():
+def _norm(model_cfg=None):
+    """BatchNorm1d as the reference has it, or, with NORM_GROUPS in the model config, a group norm of that many groups per frame (no
+    statistics over the batch, nothing to synchronise between ranks)"""
+    groups = model_cfg.get('NORM_GROUPS', None) if model_cfg is not None and hasattr(model_cfg, 'get') else None
+    if groups:
+        return partial(spconv.SparseGroupNorm, int(groups))
     return partial(nn.BatchNorm1d, eps=BN_EPS, momentum=BN_MOMENTUM)
 
 
@@ -69,12 +74,11 @@ class SparseBasicBlock(spconv.SparseModule):
         self.stride = stride
 
     def forward(self, x):
-        from .spconv.pytorch.norm import bn_act      # fused BN (+ identity) + ReLU in training mode, the modules themselves otherwise
-        out = self.conv1(x)
-        out = out.replace_feature(bn_act(out.features, self.bn1, relu=True))
+        from .spconv.pytorch.norm import norm_act    # fused norm (+ identity) + ReLU; BatchNorm outside training: the modules themselves
+        out = norm_act(self.conv1(x), self.bn1)
         out = self.conv2(out)
         identity = x if self.downsample is None else self.downsample(x)
-        return out.replace_feature(bn_act(out.features, self.bn2, residual=identity.features, relu=True))
+        return norm_act(out, self.bn2, residual=identity.features)
 
 
 def _sparse_shape(grid_size):
@@ -92,7 +96,7 @@ class _Backbone8x(nn.Module):
         super().__init__()
         assert input_channels is not None and grid_size is not None
         self.model_cfg = model_cfg
-        norm_fn = _norm()
+        norm_fn = _norm(model_cfg)
         self.sparse_shape = _sparse_shape(grid_size)
         c0 = self.STAGES[0][2]
         self.conv_input = spconv.SparseSequential(
@@ -217,7 +221,7 @@ class VoxelResBackBone8xVoxelNeXt(nn.Module):
         assert input_channels is not None and grid_size is not None
         self.model_cfg = model_cfg
         get = model_cfg.get if model_cfg is not None and hasattr(model_cfg, 'get') else (lambda k, d: d)
-        norm_fn = _norm()
+        norm_fn = _norm(model_cfg)
         ks = get('SPCONV_KERNEL_SIZES', [3, 3, 3, 3])
         ch = get('CHANNELS', [16, 32, 64, 128, 128])
         out_channel = get('OUT_CHANNEL', 128)
@@ -239,8 +243,8 @@ class VoxelResBackBone8xVoxelNeXt(nn.Module):
             spconv.SparseConv2d(ch[3], out_channel, 3, stride=1, padding=1, bias=False, indice_key='spconv_down2'),
             norm_fn(out_channel), nn.ReLU())
         self.shared_conv = spconv.SparseSequential(
-            spconv.SubMConv2d(out_channel, out_channel, 3, stride=1, padding=1, bias=True), nn.BatchNorm1d(out_channel),
-            nn.ReLU(True))
+            spconv.SubMConv2d(out_channel, out_channel, 3, stride=1, padding=1, bias=True),
+            norm_fn(out_channel) if get('NORM_GROUPS', None) else nn.BatchNorm1d(out_channel), nn.ReLU(True))
         self.forward_ret_dict = {}
         self.num_point_features = out_channel
         self.backbone_channels = {'x_conv1': ch[0], 'x_conv2': ch[1], 'x_conv3': ch[2], 'x_conv4': ch[3]}

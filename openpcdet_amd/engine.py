@@ -27,6 +27,7 @@ from . import _lib
 from .backbones import SparseBasicBlock
 from .spconv.pytorch.conv import SparseConvolution
 from .spconv.pytorch.modules import SparseSequential
+from .spconv.pytorch.norm import SparseGroupNorm
 
 
 def _fold_bn(bn, cout, device):
@@ -60,6 +61,9 @@ def _flatten_backbone(backbone):
         relu = any(isinstance(m, nn.ReLU) for m in mods[1:])
         return _ConvSpec(mods[0], bn, relu, False)
 
+    if any(isinstance(m, SparseGroupNorm) for m in backbone.modules()):
+        raise TypeError("the plan folds BatchNorm into its convolutions; a group norm's statistics are those of the frame at hand: "
+                        "run this backbone through its modules")
     stages = [[('conv', seq_conv(backbone.conv_input))]]
     for name in ('conv1', 'conv2', 'conv3', 'conv4'):
         items = []

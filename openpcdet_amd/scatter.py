@@ -2,8 +2,12 @@
 (pcdet/models/backbones_3d/vfe/dynamic_pillar_vfe.py:5-9,40,105; dynamic_mean_vfe.py:65).  Same call shape
 (`scatter_mean(src, index, dim=0)`, `scatter_max(src, index, dim=0) -> (values, argmax)`), backed by
 pvx_scatter_mean / pvx_scatter_max; both are differentiable (PFN weights train through scatter_max).
-`index` may be int32 or int64; negative entries are skipped.  `dim_size` avoids the host read of index.max()."""
+`index` may be int32 or int64; negative entries are skipped.  `dim_size` avoids the host read of index.max().
+
+`lookup_rows` is the way back, rows of a table picked by index (times a scale), with the table's gradient summed by sorted index
+(pvx_lookup_rows, pvx_sort_index, pvx_lookup_rows_grad); `sort_index` hands that sort out, for an index that several calls share."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -78,3 +82,105 @@ def scatter_max(src, index, dim=0, out=None, dim_size=None):
     v, a = _ScatterMax.apply(s, i, m)
     shape = (m,) + tuple(src.shape[1:])
     return v.reshape(shape).to(src.dtype), a.reshape(shape).long()
+
+
+# ---- rows by index -------------------------------------------------------------------------------------------------------
+class IndexSort:
+    """What `sort_index` returns for an index of n entries into num_rows rows: `order` [n] int32, the positions by ascending index
+    (equal ones by position, entries outside the rows at the end), `keys` [n] int32, the sorted indices (num_rows for those outside), and
+    `offsets` [num_rows + 1] int32: row v was named by the positions order[offsets[v]:offsets[v + 1]]."""
+
+    def __init__(self, order, keys, offsets, num_rows):
+        self.order, self.keys, self.offsets, self.num_rows = order, keys, offsets, num_rows
+
+
+def _check_index(index):
+    if not index.is_cuda:
+        raise RuntimeError("rows are looked up on the GPU only (no CPU fallback): got an index on %s" % index.device)
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TypeError("index must be int32 or int64, got %s" % index.dtype)
+
+
+def sort_index(index, num_rows):
+    """stable sort of `index` (int32 or int64, any shape, flattened) into runs of equal entries -> IndexSort; no host read"""
+    _check_index(index)
+    num_rows = int(num_rows)
+    if num_rows < 1:
+        raise ValueError("num_rows must be at least 1, got %d" % num_rows)
+    index = index.reshape(-1).contiguous()
+    n, dev = index.shape[0], index.device
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        order = torch.empty(n, dtype=torch.int32, device=dev)
+        keys = torch.empty(n, dtype=torch.int32, device=dev)
+        offsets = torch.empty(num_rows + 1, dtype=torch.int32, device=dev)
+        ws = _lib.workspace(L.pvx_sort_index_workspace_bytes(n), dev)
+        _lib.check(L.pvx_sort_index(_lib.ptr(index), int(index.dtype == torch.int64), n, num_rows, _lib.ptr(order), _lib.ptr(keys),
+                                    _lib.ptr(offsets), _lib.ptr(ws), ws.numel(), _lib.stream()), "pvx_sort_index")
+    return IndexSort(order, keys, offsets, num_rows)
+
+
+def _lookup(table, index, scale):
+    """table [m, w] contiguous, index [n] contiguous -> [n, w]"""
+    n, (m, w) = index.shape[0], table.shape
+    with torch.cuda.device(table.device):
+        out = torch.empty((n, w), dtype=table.dtype, device=table.device)
+        _lib.check(_lib.lib().pvx_lookup_rows(_lib.ptr(table), _lib.DTYPE_CODE[table.dtype], _lib.ptr(index), int(index.dtype == torch.int64),
+                                              n, m, w, scale, _lib.ptr(out), _lib.stream()), "pvx_lookup_rows")
+    return out
+
+
+class _LookupRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale, sort):
+        ctx.save_for_backward(index)
+        ctx.scale, ctx.sort, ctx.shape = scale, sort, table.shape
+        return _lookup(table, index, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        index, = ctx.saved_tensors
+        m, w = ctx.shape
+        n, dev = index.shape[0], index.device
+        grad = grad.contiguous()
+        dtable = torch.empty((m, w), dtype=grad.dtype, device=dev)
+        if m > 0 and w > 0:
+            sort = ctx.sort if ctx.sort is not None else sort_index(index, m)
+            L = _lib.lib()
+            with torch.cuda.device(dev):
+                ws = _lib.workspace(L.pvx_lookup_rows_grad_workspace_bytes(n, w), dev)
+                _lib.check(L.pvx_lookup_rows_grad(_lib.ptr(grad), _lib.DTYPE_CODE[grad.dtype], _lib.ptr(sort.order), _lib.ptr(sort.keys),
+                                                  _lib.ptr(sort.offsets), n, m, w, ctx.scale, _lib.ptr(dtable), _lib.ptr(ws), ws.numel(),
+                                                  _lib.stream()), "pvx_lookup_rows_grad")
+        return dtable, None, None, None
+
+
+def lookup_rows(table, index, scale=1.0, sort=None):
+    """scale * table[index]: table [m, ...] float32 / float16 / bfloat16, index int32 or int64 of any shape -> [*index.shape, ...] in the
+    table's dtype.  Entries outside [0, m) give zeros and pass no gradient.  The gradient with respect to the table (and only to it) adds
+    each row's entries in their order, in 32 bits, without atomics.  `sort`: sort_index(index, m) of this very index, where the caller
+    has it (the backward sorts otherwise)."""
+    if not table.is_cuda:
+        raise RuntimeError("rows are looked up on the GPU only (no CPU fallback): got a table on %s" % table.device)
+    _check_index(index)
+    if table.device != index.device:
+        raise RuntimeError("table and index are on different devices: %s and %s" % (table.device, index.device))
+    if table.dtype not in _lib.DTYPE_CODE:
+        raise TypeError("unsupported table dtype %s" % table.dtype)
+    if table.dim() < 1:
+        raise ValueError("table must have a dimension of rows")
+    if sort is not None and (sort.num_rows != table.shape[0] or sort.order.shape[0] != index.numel() or sort.order.device != table.device):
+        raise ValueError("sort is that of another index: %d entries into %d rows, wanted %d into %d"
+                         % (sort.order.shape[0], sort.num_rows, index.numel(), table.shape[0]))
+    shape = tuple(index.shape) + tuple(table.shape[1:])
+    width = 1
+    for d in table.shape[1:]:
+        width *= d
+    flat = table.reshape(table.shape[0], width).contiguous()
+    idx = index.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and flat.requires_grad:
+        out = _LookupRows.apply(flat, idx, float(scale), sort)
+    else:
+        out = _lookup(flat, idx, float(scale))
+    return out.view(shape)

@@ -5,3 +5,4 @@ from .conv import (SparseConv2d, SparseConv3d, SparseConvolution, SparseInverseC
                    SubMConv2d, SubMConv3d)
 from .core import ConvAlgo, SparseConvTensor  # noqa: F401
 from .modules import SparseModule, SparseSequential, ToDense  # noqa: F401
+from .norm import SparseGroupNorm  # noqa: F401

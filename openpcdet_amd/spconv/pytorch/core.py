@@ -118,6 +118,7 @@ class SparseConvTensor:
         self.force_algo = force_algo
         self.int8_scale = None
         self._index_holder = [None]   # shared by replace_feature() copies: one site index per coordinate set
+        self._sample_holder = [None]  # and one list of the rows of each sample
         assert features.dim() == 2 and indices.dim() == 2, "features must be [N, C], indices [N, 1 + ndim]"
         assert indices.shape[1] == len(self.spatial_shape) + 1, "indices must have 1 + ndim columns"
         assert indices.dtype == torch.int32, "indices must be int32 (pass coords.int())"
@@ -209,6 +210,17 @@ class SparseConvTensor:
 
     def _seed_site_index(self, index, perm, n_unique):
         self._index_holder[0] = _SiteIndexCache(self.indices, index, perm, n_unique)
+
+    def _sample_rows(self):
+        """(offsets [batch_size + 1], order [N], both int32): sample b has the rows order[offsets[b]:offsets[b + 1]], in ascending order;
+        rows whose batch index is outside the batch come last.  Kept like the site index."""
+        c = self._sample_holder[0]
+        if c is not None and c[0].valid_for(self.indices):
+            return c[1], c[2]
+        from ...scatter import sort_index
+        s = sort_index(self.indices[:, 0], self.batch_size)
+        self._sample_holder[0] = (_SiteIndexCache(self.indices, None, None, None), s.offsets, s.order)
+        return s.offsets, s.order
 
     # ---- dense() --------------------------------------------------------------------------------------
     def dense(self, channels_first=True):

@@ -70,7 +70,12 @@ class SparseSequential(SparseModule):
             module = mods[i]
             if is_spconv_module(module):
                 assert isinstance(input, SparseConvTensor)
-                input = module(input)
+                act = norm.act_name(mods[i + 1]) if isinstance(module, norm.SparseGroupNorm) and i + 1 < len(mods) else None
+                if act is not None:     # the activation behind a group norm runs in its kernels
+                    input = module(input, act=act)
+                    i += 1
+                else:
+                    input = module(input)
             elif isinstance(input, SparseConvTensor):
                 if input.indices.shape[0] != 0:
                     # BatchNorm1d -> ReLU in training mode: one fused op (csrc/batchnorm.hip) instead of six torch launches

@@ -2,14 +2,20 @@
 `norm_fn(C) -> nn.ReLU()` (pcdet/models/backbones_3d/spconv_backbone.py:21-25) and `bn -> += identity -> relu` (:52-64) compute,
 on csrc/batchnorm.hip.  The modules stay plain `nn.BatchNorm1d` / `nn.ReLU` (state-dict keys, `.eval()`, SyncBatchNorm conversion
 all unchanged); `SparseSequential` and `SparseBasicBlock` call `bn_act` where they see the pattern.  Anything the kernels do not
-take -- eval mode, SyncBatchNorm, momentum=None, CPU tensors, odd channel counts -- goes through the modules themselves."""
+take -- eval mode, SyncBatchNorm, momentum=None, CPU tensors, odd channel counts -- goes through the modules themselves.
+
+Group norm (+ residual) + activation over the rows of each sample, `group_norm_act` and the module `SparseGroupNorm`, is the
+normalisation that needs no batch and no all-reduce (csrc/group_norm.hip); the same in training and in evaluation."""
 import os
 
 import torch
 from torch import nn
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from ... import _lib
+from .core import SparseConvTensor
+from .modules import SparseModule
 
 _ENABLED = os.environ.get("PVX_FUSED_BN", "1") != "0"       # A/B switch
 
@@ -162,3 +168,174 @@ def bn_act(x, bn, residual=None, relu=True):
                 y = y + residual
             return torch.relu(y) if relu else y
     return _BNAct.apply(*args)
+
+
+# ---- group norm ------------------------------------------------------------------------------------------------------------
+_ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def act_name(module):
+    """the name `group_norm_act` has for an activation module, None if it has none"""
+    if type(module) is nn.ReLU:
+        return "relu"
+    if type(module) is nn.SiLU:
+        return "silu"
+    if type(module) is nn.GELU and module.approximate == "none":
+        return "gelu"
+    return None
+
+
+def _group_norm_fwd(x, weight, bias, residual, offsets, order, samples, groups, eps, act):
+    """x [n, c] contiguous -> y, mean, rstd"""
+    L = _lib.lib()
+    n, c = x.shape
+    dev = x.device
+    with torch.cuda.device(dev):
+        y = torch.empty_like(x)
+        stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
+        ws = _lib.workspace(L.pvx_group_norm_act_workspace_bytes(n, c, samples, int(offsets is not None), groups), dev)
+        base = stats.data_ptr()
+        _lib.check(L.pvx_group_norm_act_fwd(_lib.ptr(x), n, c, _lib.DTYPE_CODE[x.dtype], samples, _lib.ptr(offsets), _lib.ptr(order), groups,
+                                            _lib.ptr(weight), _lib.ptr(bias), _param_code(weight, bias), eps, _lib.ptr(residual), act,
+                                            _lib.ptr(y), base, base + 4 * samples * groups, _lib.ptr(ws), ws.numel(), _lib.stream()),
+                   "pvx_group_norm_act_fwd")
+    return y, stats
+
+
+def _param_code(weight, bias):
+    p = weight if weight is not None else bias
+    return _lib.DTYPE_CODE[p.dtype] if p is not None else _lib.PVX_F32
+
+
+class _GroupNormAct(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, offsets, order, samples, groups, eps, act):
+        y, stats = _group_norm_fwd(x, weight, bias, residual, offsets, order, samples, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, residual, offsets, order, stats)
+        ctx.args = (samples, groups, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, residual, offsets, order, stats = ctx.saved_tensors
+        samples, groups, act = ctx.args
+        L = _lib.lib()
+        n, c = x.shape
+        dev = x.device
+        dy = dy.contiguous()
+        with torch.cuda.device(dev):
+            dx = torch.empty_like(x)
+            dres = torch.empty_like(x) if residual is not None else None
+            dw = torch.empty_like(weight) if weight is not None else None
+            db = torch.empty_like(bias) if bias is not None else None
+            ws = _lib.workspace(L.pvx_group_norm_act_workspace_bytes(n, c, samples, int(offsets is not None), groups), dev)
+            base = stats.data_ptr()
+            _lib.check(L.pvx_group_norm_act_bwd(_lib.ptr(dy), _lib.ptr(x), _lib.ptr(residual), n, c, _lib.DTYPE_CODE[x.dtype], samples,
+                                                _lib.ptr(offsets), _lib.ptr(order), groups, _lib.ptr(weight), _lib.ptr(bias),
+                                                _param_code(weight, bias), base, base + 4 * samples * groups, act, _lib.ptr(dx), _lib.ptr(dres),
+                                                _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), ws.numel(), _lib.stream()),
+                       "pvx_group_norm_act_bwd")
+        return dx, dw, db, dres, None, None, None, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, residual=None, offsets=None, order=None):
+    """act(group_norm(x) (+ residual)), channels last.
+
+    x [B, ..., C]: each x[b] is a sample and its statistics go over every position of it and the C / num_groups channels of a group (what
+    torch.nn.functional.group_norm computes with the channels moved to dimension 1).  With `offsets` (int32 [B + 1], device, ascending),
+    x is [N, C] and sample b owns the positions offsets[b]:offsets[b + 1]; position p is row p, or row order[p] (`order`: int32 [N], a
+    permutation).  Rows at positions of no sample get zeros, and a zero gradient.
+
+    x float32 / float16 / bfloat16; weight and bias [C] of one dtype of these; residual like x; act None, "relu", "silu" or "gelu" (with
+    the error function).  Gradients with respect to x, weight, bias and residual.  One kernel where each sample is known to fit a
+    workgroup, three otherwise; the same bits on every run."""
+    if not x.is_cuda:
+        raise RuntimeError("group_norm_act runs on the GPU only (no CPU fallback): got a tensor on %s" % x.device)
+    if x.dtype not in _lib.DTYPE_CODE:
+        raise TypeError("unsupported dtype %s" % x.dtype)
+    if x.dim() < 2:
+        raise ValueError("x must be [B, ..., C], got %s" % (tuple(x.shape),))
+    if act not in _ACTS:
+        raise ValueError("act must be one of None, 'relu', 'silu', 'gelu', got %r" % (act,))
+    c, num_groups, eps = x.shape[-1], int(num_groups), float(eps)
+    if num_groups < 1 or c < 1 or c % num_groups != 0:
+        raise ValueError("%d channels do not make %d groups" % (c, num_groups))
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative, got %r" % (eps,))
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if tuple(p.shape) != (c,) or p.device != x.device:
+            raise ValueError("%s must be [%d] on %s, got %s on %s" % (name, c, x.device, tuple(p.shape), p.device))
+        if p.dtype not in _lib.DTYPE_CODE or (weight is not None and p.dtype != weight.dtype):
+            raise TypeError("weight and bias must share one of float32, float16 and bfloat16, got %s for %s" % (p.dtype, name))
+    if residual is not None:
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ValueError("residual must be %s on %s, got %s on %s" % (tuple(x.shape), x.device, tuple(residual.shape), residual.device))
+        residual = residual.to(x.dtype)
+    if offsets is None:
+        if order is not None:
+            raise ValueError("order needs offsets")
+        samples = x.shape[0]
+    else:
+        if x.dim() != 2:
+            raise ValueError("with offsets, x must be [N, C], got %s" % (tuple(x.shape),))
+        for name, t, shape in (("offsets", offsets, None), ("order", order, (x.shape[0],))):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or t.dim() != 1 or t.device != x.device or (shape is not None and tuple(t.shape) != shape):
+                raise ValueError("%s must be an int32 vector%s on %s, got %s %s on %s" % (
+                    name, " of %d" % shape if shape else "", x.device, t.dtype, tuple(t.shape), t.device))
+        samples = offsets.shape[0] - 1
+        if samples < 1:
+            raise ValueError("offsets must have an entry more than there are samples")
+        offsets = offsets.contiguous()
+        order = order.contiguous() if order is not None else None
+    flat = x.reshape(-1, c).contiguous()
+    if flat.shape[0] == 0:
+        samples = max(samples, 1)
+    res = residual.reshape(-1, c).contiguous() if residual is not None else None
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    args = (flat, w, b, res, offsets, order, samples, num_groups, eps, _ACTS[act])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        y = _GroupNormAct.apply(*args)
+    else:
+        y = _group_norm_fwd(*args)[0]
+    return y.view(x.shape)
+
+
+class SparseGroupNorm(SparseModule):
+    """GroupNorm over a SparseConvTensor: statistics over the sites of each sample (frame) and the channels of a group.  Parameters are
+    those of nn.GroupNorm (`weight`, `bias`).  In a SparseSequential a ReLU, SiLU or GELU behind it runs in the same kernels.  (nn.GroupNorm
+    itself, given the [N, C] features, takes every site for a sample of its own.)"""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, device=None, dtype=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups != 0:
+            raise ValueError("%d channels do not make %d groups" % (num_channels, num_groups))
+        self.num_groups, self.num_channels, self.eps, self.affine = int(num_groups), int(num_channels), float(eps), bool(affine)
+        if affine:
+            self.weight = nn.Parameter(torch.ones(num_channels, device=device, dtype=dtype))
+            self.bias = nn.Parameter(torch.zeros(num_channels, device=device, dtype=dtype))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def extra_repr(self):
+        return "{num_groups}, {num_channels}, eps={eps}, affine={affine}".format(**self.__dict__)
+
+    def forward(self, input, act=None, residual=None):
+        """act(norm(input) (+ residual)); residual: features of the same sites"""
+        assert isinstance(input, SparseConvTensor), "expected a SparseConvTensor"
+        offsets, order = input._sample_rows()
+        return input.replace_feature(group_norm_act(input.features, self.num_groups, self.weight, self.bias, self.eps, act, residual,
+                                                    offsets, order))
+
+
+def norm_act(x, norm, residual=None, relu=True):
+    """relu?(norm(x) (+ residual)) for a SparseConvTensor x and a norm of either kind -> SparseConvTensor"""
+    if isinstance(norm, SparseGroupNorm):
+        return norm(x, act="relu" if relu else None, residual=residual)
+    return x.replace_feature(bn_act(x.features, norm, residual=residual, relu=relu))

@@ -23,7 +23,7 @@ from torch import nn
 import torch.nn.functional as F
 
 from . import _lib
-from .scatter import scatter_max, scatter_mean
+from .scatter import lookup_rows, scatter_max, scatter_mean
 
 
 def _ns(cfg):
@@ -140,7 +140,9 @@ class PFNLayerV2(nn.Module):
         x_max = scatter_max(x, unq_inv, dim=0, dim_size=num_voxels)[0]
         if self.last_vfe:
             return x_max
-        return torch.cat([x, x_max[unq_inv.long(), :]], dim=1)
+        if x_max.dtype not in _lib.DTYPE_CODE or unq_inv.dtype not in (torch.int32, torch.int64):
+            return torch.cat([x, x_max[unq_inv.long(), :]], dim=1)
+        return torch.cat([x, lookup_rows(x_max, unq_inv)], dim=1)
 
 
 class _DynamicPFNVFE(_VFEBase):

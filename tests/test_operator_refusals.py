@@ -1,0 +1,83 @@
+"""CPU: what the training-step operators refuse before anything is launched, at the C entries (codes, never an abort) and in Python."""
+import pytest
+import torch
+
+from openpcdet_amd import _lib, scatter
+from openpcdet_amd.spconv import pytorch as spconv
+from openpcdet_amd.spconv.pytorch import norm
+
+INVALID, WORKSPACE, RANGE = -1, -2, -4
+P = 4096          # stands for a device address: refused calls never follow it
+
+
+def fwd(**kw):
+    a = dict(x=P, n=10, c=8, dtype=0, samples=2, offsets=P, order=None, groups=2, weight=P, bias=P, pd=0, eps=1e-5, residual=None, act=1, y=P,
+             mean=P, rstd=P, ws=P, size=0)
+    a.update(kw)
+    return _lib.lib().pvx_group_norm_act_fwd(*[a[k] for k in ("x", "n", "c", "dtype", "samples", "offsets", "order", "groups", "weight", "bias",
+                                                             "pd", "eps", "residual", "act", "y", "mean", "rstd", "ws", "size")], None)
+
+
+def bwd(**kw):
+    a = dict(dy=P, x=P, residual=None, n=10, c=8, dtype=0, samples=2, offsets=P, order=None, groups=2, weight=P, bias=P, pd=0, mean=P, rstd=P,
+             act=1, dx=P, dres=None, dw=P, db=P, ws=P, size=0)
+    a.update(kw)
+    return _lib.lib().pvx_group_norm_act_bwd(*[a[k] for k in ("dy", "x", "residual", "n", "c", "dtype", "samples", "offsets", "order", "groups",
+                                                             "weight", "bias", "pd", "mean", "rstd", "act", "dx", "dres", "dw", "db", "ws",
+                                                             "size")], None)
+
+
+def test_group_norm_codes():
+    for call in (fwd, bwd):
+        for kw in (dict(n=-1), dict(c=0), dict(c=-8), dict(samples=0), dict(groups=0), dict(groups=3), dict(dtype=3), dict(dtype=-1), dict(pd=7),
+                   dict(act=4), dict(act=-1), dict(x=None), dict(mean=None), dict(rstd=None), dict(offsets=None, samples=3)):
+            assert call(**kw) == INVALID, kw
+        assert call() == WORKSPACE and call(ws=None, size=1 << 30) == WORKSPACE
+        assert call(n=0x7fffffff) == RANGE and call(c=1 << 21, groups=1) == RANGE and call(samples=0x7fffffff, groups=2) == RANGE
+    assert fwd(y=None) == INVALID and fwd(eps=-1.0) == INVALID and fwd(eps=float("nan")) == INVALID
+    assert bwd(dy=None) == INVALID and bwd(dx=None) == INVALID
+    assert fwd(n=0) == 0 and bwd(n=0, dw=None, db=None) == 0
+    L = _lib.lib()
+    small, large = L.pvx_group_norm_act_workspace_bytes(1000, 16, 2, 1, 4), L.pvx_group_norm_act_workspace_bytes(10 ** 6, 64, 5000, 1, 8)
+    assert 256 < small < large and L.pvx_group_norm_act_workspace_bytes(0, 16, 2, 1, 4) == 256
+    assert fwd(ws=P, size=L.pvx_group_norm_act_workspace_bytes(10, 8, 2, 1, 2) - 256) == WORKSPACE
+
+
+def test_lookup_codes():
+    L = _lib.lib()
+    look = lambda table=P, dtype=0, index=P, wide=0, n=5, m=4, w=8, out=P: L.pvx_lookup_rows(table, dtype, index, wide, n, m, w, 1.0, out, None)  # noqa: E731
+    for kw in (dict(n=-1), dict(m=-1), dict(w=-1), dict(dtype=3), dict(dtype=-1), dict(table=None), dict(index=None), dict(out=None)):
+        assert look(**kw) == INVALID, kw
+    assert look(n=0) == 0 and look(w=0) == 0 and look(n=0x7fffffff) == RANGE and look(m=0x7fffffff) == RANGE and look(w=1 << 25) == RANGE
+    sort = lambda index=P, n=5, m=4, order=P, keys=P, offsets=P, ws=P, size=0: L.pvx_sort_index(index, 1, n, m, order, keys, offsets, ws, size, None)  # noqa: E731
+    for kw in (dict(n=-1), dict(m=0), dict(m=-2), dict(index=None), dict(order=None), dict(keys=None), dict(offsets=None)):
+        assert sort(**kw) == INVALID, kw
+    assert sort(n=0x7fffffff) == RANGE and sort(m=0x7fffffff) == RANGE
+    assert sort(n=100000, m=50) == WORKSPACE and sort(n=100000, ws=None, size=1 << 30) == WORKSPACE
+    assert L.pvx_sort_index_workspace_bytes(100000) > 3 * 4 * 100000 and L.pvx_sort_index_workspace_bytes(0) == 256
+    grad = lambda dout=P, dtype=0, order=P, keys=P, offsets=P, n=5000, m=4, w=8, out=P, ws=P, size=0: L.pvx_lookup_rows_grad(  # noqa: E731
+        dout, dtype, order, keys, offsets, n, m, w, 1.0, out, ws, size, None)
+    for kw in (dict(n=-1), dict(m=-1), dict(w=-1), dict(dtype=9), dict(dout=None), dict(order=None), dict(keys=None), dict(offsets=None), dict(out=None)):
+        assert grad(**kw) == INVALID, kw
+    assert grad(m=0) == 0 and grad(w=0) == 0 and grad() == WORKSPACE and grad(n=0x7fffffff) == RANGE
+    assert L.pvx_lookup_rows_grad_workspace_bytes(5000, 8) > 5000 // 32 * 8 * 4
+
+
+def test_python_refuses_cpu_tensors():
+    x = torch.zeros(6, 8)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        norm.group_norm_act(x, 2)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        scatter.lookup_rows(x, torch.zeros(3, dtype=torch.long))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        scatter.sort_index(torch.zeros(3, dtype=torch.long), 4)
+
+
+def test_modules_refuse():
+    with pytest.raises(ValueError):
+        spconv.SparseGroupNorm(3, 16)
+    with pytest.raises(ValueError):
+        spconv.SparseGroupNorm(0, 16)
+    gn = spconv.SparseGroupNorm(4, 16, affine=False)
+    assert list(gn.parameters()) == [] and "4, 16" in repr(gn)
+    assert norm.act_name(torch.nn.GELU("tanh")) is None and norm.act_name(torch.nn.GELU()) == "gelu" and norm.act_name(torch.nn.ReLU6()) is None
