@@ -576,6 +576,19 @@ int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, 
                            void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ----------------------------------------------------------------------------------------------------
+ * Orthogonalisation of weight updates by Newton-Schulz steps (the update of the Muon optimiser), for up to PVX_ORTHO_MAX matrices of
+ * one dtype in one call.  Each matrix, taken as X with no more rows than columns (transposed if need be):
+ *   X = M / (|M|_F + eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X;   out = X in the matrix's own orientation
+ * mats: HOST array; in and out are device pointers to contiguous row-major matrices (they may be the same).  f32 matrices are
+ * multiplied with the accuracy of binary32, 16-bit ones with about 17 bits; sums are binary32.  rows, cols <= 2^20.
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct { const void* in; void* out; int rows, cols; } pvx_matrix;
+#define PVX_ORTHO_MAX 64
+size_t pvx_orthogonalize_workspace_bytes(const pvx_matrix* mats, int count, int dtype);
+int pvx_orthogonalize(const pvx_matrix* mats, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------------------------
  * Point-level preparation ahead of the voxelizer: the world augmentations and the range mask /
  * shuffle the reference runs with numpy in DataLoader workers.  binary32 arithmetic in the reference's order (numpy 1.x casting:
  * the drawn float64 scalars act as float32), no contraction.

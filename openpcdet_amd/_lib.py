@@ -63,6 +63,8 @@ SIGNATURES = {
     "pvx_group_norm_act_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                        c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                        c_size_t, c_void_p]),
+    "pvx_orthogonalize_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int]),
+    "pvx_orthogonalize": (c_int, [c_void_p, c_int, c_int, c_int, c_float, c_float, c_float, c_float, c_void_p, c_size_t, c_void_p]),
     "pvx_points_transform": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "pvx_boxes_transform": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "pvx_points_prepare_workspace_bytes": (c_size_t, [c_int]),

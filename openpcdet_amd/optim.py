@@ -1,0 +1,123 @@
+"""Orthogonalised updates for the training step: `orthogonalize` (Newton-Schulz steps on the GPU's matrix cores, many weights in one
+call: pvx_orthogonalize) and `Muon`, the optimiser that applies them to momentum.
+
+A convolution weight [Cout, kz, ky, kx, Cin] is the matrix [Cout, kz ky kx Cin] it multiplies unfolded features with.  `Muon` takes the
+weights of two and more dimensions; norms, biases and the like belong to another optimiser (the training step's AdamW), and so does
+the exchange of gradients between ranks (`dist.allreduce_gradients`, DistributedDataParallel): every rank makes the same update from
+the averaged gradient."""
+import struct
+
+import torch
+
+from . import _lib
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # a s + b s^3 + c s^5: steepest at 0 of those that keep (0, 1] within about 0.7 .. 1.2
+MAX_MATRICES = 64                             # PVX_ORTHO_MAX
+
+
+def _launch(mats, outs, steps, coefficients, eps):
+    """mats, outs: contiguous matrices of one dtype on one device, none of them empty"""
+    L = _lib.lib()
+    dev, code = mats[0].device, _lib.DTYPE_CODE[mats[0].dtype]
+    a, b, c = coefficients
+    with torch.cuda.device(dev):
+        stream = _lib.stream()
+        for at in range(0, len(mats), MAX_MATRICES):
+            part = [v for m, o in zip(mats[at:at + MAX_MATRICES], outs[at:at + MAX_MATRICES]) for v in (m.data_ptr(), o.data_ptr(), *m.shape)]
+            count = len(part) // 4
+            table = struct.pack("QQii" * count, *part)
+            ws = _lib.workspace(L.pvx_orthogonalize_workspace_bytes(table, count, code), dev)
+            _lib.check(L.pvx_orthogonalize(table, count, code, steps, a, b, c, eps, _lib.ptr(ws), ws.numel(), stream), "pvx_orthogonalize")
+
+
+def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """Newton-Schulz orthogonalisation: each matrix M becomes X after `steps` times X <- a X + (b A + c A A) X with A = X X^T, from
+    X = M / (|M|_F + eps) (with the shorter side first), (a, b, c) = coefficients: the singular vectors of M with singular values near 1.
+
+    matrices: a matrix [r, c], a batch of them [B, r, c], or a list or tuple of matrices of any sizes; float32 / float16 / bfloat16, on the
+    GPU.  The result has the same form, in the inputs' dtypes: binary32 matrices are computed in binary32 accuracy, 16-bit ones a little
+    above their own.  No gradient flows through it.  Matrices of one dtype go through the GPU together, up to 64 in a call."""
+    one = isinstance(matrices, torch.Tensor)
+    if one and matrices.dim() not in (2, 3):
+        raise ValueError("a matrix [r, c] or a batch [B, r, c] is wanted, got %s" % (tuple(matrices.shape),))
+    if len(coefficients) != 3:
+        raise ValueError("three coefficients are wanted, got %d" % len(coefficients))
+    steps, eps, coefficients = int(steps), float(eps), tuple(float(v) for v in coefficients)
+    if steps < 0 or not eps >= 0.0:
+        raise ValueError("steps and eps must not be negative, got %r and %r" % (steps, eps))
+    with torch.no_grad():
+        mats = list(matrices.detach().contiguous().unbind(0)) if one and matrices.dim() == 3 else [matrices] if one else list(matrices)
+        groups, outs = {}, []
+        for m in mats:
+            if not isinstance(m, torch.Tensor) or m.dim() != 2:
+                raise ValueError("matrices are wanted, got %s" % (tuple(m.shape) if isinstance(m, torch.Tensor) else type(m).__name__,))
+            if not m.is_cuda:
+                raise RuntimeError("orthogonalize runs on the GPU only (no CPU fallback): got a matrix on %s" % m.device)
+            if m.dtype not in _lib.DTYPE_CODE:
+                raise TypeError("unsupported dtype %s" % m.dtype)
+        if one and matrices.dim() == 3:
+            whole = torch.empty(matrices.shape, dtype=matrices.dtype, device=matrices.device)
+            outs = list(whole.unbind(0))
+        else:
+            outs = [torch.empty(m.shape, dtype=m.dtype, device=m.device) for m in mats]
+        for m, o in zip(mats, outs):
+            if m.numel() > 0:
+                g = groups.setdefault((m.dtype, m.device), ([], []))
+                g[0].append(m.contiguous())
+                g[1].append(o)
+        for g in groups.values():
+            _launch(g[0], g[1], steps, coefficients, eps)
+    if one:
+        return whole if matrices.dim() == 3 else outs[0]
+    return type(matrices)(outs) if isinstance(matrices, (list, tuple)) and type(matrices) in (list, tuple) else outs
+
+
+class Muon(torch.optim.Optimizer):
+    """momentum buf <- momentum buf + grad; update = orthogonalize(grad + momentum buf, or buf without nesterov);
+    p <- (1 - lr weight_decay) p - lr max(1, rows / cols)^0.5 update, for parameters of two and more dimensions taken as the matrix
+    [shape[0], everything else].  All matrices of a step are orthogonalised together."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+        if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
+            raise ValueError("lr and weight_decay must not be negative and momentum must be in [0, 1): got %r, %r, %r" % (lr, weight_decay, momentum))
+        if int(steps) < 0 or not eps >= 0.0 or len(coefficients) != 3:
+            raise ValueError("steps and eps must not be negative, with three coefficients: got %r, %r, %r" % (steps, eps, coefficients))
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps),
+                                      coefficients=tuple(coefficients), eps=eps))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError("Muon takes parameters of two and more dimensions, got %s: give the others to another optimiser" % (tuple(p.shape),))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None and p.numel() > 0]
+            if not params:
+                continue
+            for p in params:
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
+                if "momentum_buffer" not in self.state[p]:
+                    self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            grads = [p.grad for p in params]
+            bufs = [self.state[p]["momentum_buffer"] for p in params]
+            torch._foreach_mul_(bufs, group["momentum"])
+            torch._foreach_add_(bufs, grads)
+            updates = torch._foreach_add(grads, bufs, alpha=group["momentum"]) if group["nesterov"] else bufs
+            mats = orthogonalize([u.reshape(u.shape[0], -1) for u in updates], group["steps"], group["coefficients"], group["eps"])
+            if group["weight_decay"] != 0.0:
+                torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
+            by_scale = {}
+            for p, o in zip(params, mats):
+                by_scale.setdefault(max(1.0, o.shape[0] / o.shape[1]) ** 0.5, []).append((p, o.view(p.shape)))
+            for scale, pairs in by_scale.items():
+                torch._foreach_add_([p for p, _ in pairs], [o for _, o in pairs], alpha=-group["lr"] * scale)
+        return loss

@@ -1,8 +1,10 @@
 """CPU: what the training-step operators refuse before anything is launched, at the C entries (codes, never an abort) and in Python."""
+import struct
+
 import pytest
 import torch
 
-from openpcdet_amd import _lib, scatter
+from openpcdet_amd import _lib, optim, scatter
 from openpcdet_amd.spconv import pytorch as spconv
 from openpcdet_amd.spconv.pytorch import norm
 
@@ -81,3 +83,35 @@ def test_modules_refuse():
     gn = spconv.SparseGroupNorm(4, 16, affine=False)
     assert list(gn.parameters()) == [] and "4, 16" in repr(gn)
     assert norm.act_name(torch.nn.GELU("tanh")) is None and norm.act_name(torch.nn.GELU()) == "gelu" and norm.act_name(torch.nn.ReLU6()) is None
+
+
+def test_orthogonalize_codes():
+    L = _lib.lib()
+    call = lambda mats, count=None, dtype=0, steps=5, eps=1e-7, ws=P, size=0: L.pvx_orthogonalize(  # noqa: E731
+        struct.pack("QQii" * len(mats), *[v for m in mats for v in m]) if mats else None, len(mats) if count is None else count, dtype, steps,
+        3.4445, -4.775, 2.0315, eps, ws, size, None)
+    good = (P, P, 16, 432)
+    for args in (dict(mats=[good], count=-1), dict(mats=[], count=2), dict(mats=[good], dtype=3), dict(mats=[good], steps=-1), dict(mats=[good], eps=-1.0),
+                 dict(mats=[good], eps=float("nan")), dict(mats=[good, (P, P, 0, 4)]), dict(mats=[(P, P, 4, -1)]), dict(mats=[(0, P, 4, 4)]),
+                 dict(mats=[good, (P, 0, 4, 4)])):
+        assert call(**args) == INVALID, args
+    assert call([good] * 65) == RANGE and call([(P, P, 4, (1 << 20) + 1)]) == RANGE
+    assert call([]) == 0 and call([good]) == WORKSPACE and call([good], ws=None, size=1 << 30) == WORKSPACE
+    need = L.pvx_orthogonalize_workspace_bytes(struct.pack("QQii", *good), 1, 0)
+    assert need > 4 * 16 * 432 and call([good], size=need - 1) == WORKSPACE and call([good], ws=P + 16, size=need) == WORKSPACE
+    assert L.pvx_orthogonalize_workspace_bytes(None, 0, 0) == 256
+
+
+def test_optimiser_refuses():
+    w = torch.nn.Parameter(torch.zeros(4, 4))
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(momentum=-0.1), dict(weight_decay=-1.0), dict(steps=-1), dict(eps=-1.0), dict(coefficients=(1.0,))):
+        with pytest.raises(ValueError):
+            optim.Muon([w], **kw)
+    with pytest.raises(ValueError, match="two and more"):
+        optim.Muon([w, torch.nn.Parameter(torch.zeros(4))])
+    w.grad = torch.ones(4, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        optim.Muon([w]).step()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        optim.orthogonalize(torch.zeros(4, 4))
+    assert optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))]).step() is None      # nothing has a gradient

@@ -5,7 +5,7 @@ size = the ranks launched) -> AdamW step, on Waymo-range multi-sweep frames (too
 tools/train.py:130-131,162).  Prints ONE JSON line: ms per step, frames/s, and per-kernel-class device time with the
 useful-flop fraction of the dense bf16 MFMA peak for forward, dgrad and wgrad (flops = 2 P Cin Cout each, P = valid pairs).
 
-    python tools/bench_train.py --batch 2 --points 250000 --steps 10 [--sync-bn] [--no-ddp]
+    python tools/bench_train.py --batch 2 --points 250000 --steps 10 [--sync-bn] [--no-ddp] [--norm-groups 8] [--optimizer muon]
     python -m torch.distributed.run --nproc-per-node N --master-addr 127.0.0.1 tools/bench_train.py ...
 
 The 8-GPU half of configs[3] is the driver's to run; correctness of the N > 1 path is covered by tests/test_dist_gloo.py."""
@@ -20,7 +20,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
-from openpcdet_amd import backbones, synth, voxelize  # noqa: E402
+from openpcdet_amd import backbones, optim, synth, voxelize  # noqa: E402
 from openpcdet_amd import dist as pdist  # noqa: E402
 
 PEAK = 2500.0
@@ -35,6 +35,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--sync-bn", action="store_true")
     ap.add_argument("--no-ddp", action="store_true")
+    ap.add_argument("--norm-groups", type=int, default=0, help="group norm of this many groups per frame in place of BatchNorm")
+    ap.add_argument("--optimizer", choices=("adamw", "muon"), default="adamw", help="muon: orthogonalised updates for the convolutions, AdamW for the rest")
     ap.add_argument("--no-fused-opt", action="store_true", help="torch's default (foreach) AdamW instead of the fused one")
     args = ap.parse_args()
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
@@ -48,12 +50,17 @@ def main():
     cfg = synth.CONFIGS["waymo_centerpoint"]
     grid = [int(round((cfg["range"][3 + j] - cfg["range"][j]) / cfg["voxel"][j])) for j in range(3)]
     torch.manual_seed(5)
-    net = backbones.VoxelResBackBone8x(input_channels=cfg["C"], grid_size=np.array(grid)).to(dev).train()
+    net = backbones.VoxelResBackBone8x(input_channels=cfg["C"], grid_size=np.array(grid),
+                                       model_cfg={"NORM_GROUPS": args.norm_groups} if args.norm_groups else None).to(dev).train()
     if args.sync_bn:
         net = torch.nn.SyncBatchNorm.convert_sync_batchnorm(net)
     hc = backbones.HeightCompression()
     model = net if args.no_ddp else torch.nn.parallel.DistributedDataParallel(net, device_ids=[local_rank])
-    opt = torch.optim.AdamW(net.parameters(), lr=1e-4, fused=not args.no_fused_opt)      # one multi-tensor kernel per step
+    convs = [p for p in net.parameters() if p.dim() >= 2] if args.optimizer == "muon" else []
+    rest = [p for p in net.parameters() if not convs or p.dim() < 2]
+    opts = [torch.optim.AdamW(rest, lr=1e-4, fused=not args.no_fused_opt)]      # one multi-tensor kernel per step
+    if convs:
+        opts.append(optim.Muon(convs, lr=0.02))
     gen = voxelize.PointToVoxel(cfg["voxel"], cfg["range"], cfg["C"], cfg["max_voxels"], cfg["T"])
     clouds = []
     for b in range(args.batch):
@@ -75,10 +82,12 @@ def main():
             bd = model(bd)
             bev = hc(bd)["spatial_features"]
             loss = (bev.float() ** 2).mean()
-        opt.zero_grad(set_to_none=True)
+        for opt in opts:
+            opt.zero_grad(set_to_none=True)
         loss.backward()
         torch.nn.utils.clip_grad_norm_(net.parameters(), 10.0)      # GRAD_NORM_CLIP, train_utils.py:59-60
-        opt.step()
+        for opt in opts:
+            opt.step()
         return loss, bd
 
     for _ in range(args.warmup):
@@ -100,7 +109,8 @@ def main():
            "higher_is_better": True, "scaling": "weak", "dtype": "bf16", "data": "synthetic",
            "config": {"workload": "CenterPoint/PV-RCNN++ Waymo-range training step (BASELINE.json configs[3]): %d frames x %d points x %d sweeps, "
                                   "0.1 m voxels" % (args.batch, args.points, args.sweeps), "voxels": n_vox, "ddp": not args.no_ddp, "sync_bn": args.sync_bn,
-                      "optimizer": "AdamW" + ("" if args.no_fused_opt else " (fused)"), "grad_clip": 10.0},
+                      "norm": "group norm, %d groups" % args.norm_groups if args.norm_groups else "batch norm",
+                      "optimizer": "AdamW" + ("" if args.no_fused_opt else " (fused)") + (" + Muon" if convs else ""), "grad_clip": 10.0},
            "loss": float(loss.item()), "flops_fwd": fwd, "flops_step_fwd_dgrad_wgrad": 3 * fwd,
            "mfma_frac_whole_step": round(3 * fwd / (elapsed / args.steps) / 1e12 / PEAK, 5)}
     if rank == 0:
