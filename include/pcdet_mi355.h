@@ -579,8 +579,8 @@ int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, 
  * Orthogonalisation of weight updates by Newton-Schulz steps (the update of the Muon optimiser), for up to PVX_ORTHO_MAX matrices of
  * one dtype in one call.  Each matrix, taken as X with no more rows than columns (transposed if need be):
  *   X = M / (|M|_F + eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X;   out = X in the matrix's own orientation
- * mats: HOST array; in and out are device pointers to contiguous row-major matrices (they may be the same).  f32 matrices are
- * multiplied with the accuracy of binary32, 16-bit ones with about 17 bits; sums are binary32.  rows, cols <= 2^20.
+ * mats: HOST array; in and out are device pointers to contiguous row-major matrices (they may be the same).  The
+ * products have the accuracy of binary32, whatever the dtype.  rows, cols <= 2^20, steps <= 64.
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct { const void* in; void* out; int rows, cols; } pvx_matrix;
 #define PVX_ORTHO_MAX 64

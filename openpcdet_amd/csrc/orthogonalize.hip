@@ -1,35 +1,41 @@
 // Newton-Schulz orthogonalisation of weight updates, many matrices in one call.
 //
 // For each matrix M (transposed if it has more rows than columns, so X is m x n with m <= n):
-//   X = M / (|M|_F + eps);   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
+//   X = M / (|M|_F + eps);   steps times:  A = X X^T,  B = a I + b A + c A A,  X <- B X
 // which applies the odd polynomial a s + b s^3 + c s^5 to every singular value.
 //
-// The products run on the bf16 matrix cores with the operands split into bf16 planes: x = x0 + x1 (+ x2), each plane the rounding of
-// what the ones before it left.  binary32 matrices take three planes (24 bits) and the six products of total order <= 2, 16-bit
-// ones two planes and three products (2^-17 relative, far under their own rounding), accumulated in binary32.  The binary32 matrix
-// instruction would do one product at 1/16 of the bf16 rate; six at the full one are 2.7 times faster.  X is kept as planes, which
-// is what the next product reads, and so are A and B; nothing is rounded to fewer bits than the planes hold.
+// The products run on the f16 matrix cores with each operand split in two: x = hi + lo, hi the rounding of x to 11 bits and lo that of
+// the rest, 22 bits and more together, and three of the four products (lo lo is below 2^-24 of hi hi), accumulated in binary32.
+// Against 64 bits this is as near as binary32 products are (measured: 2.6e-6 and 3.5e-6 for 1001 x 2003), at a third of the f16
+// rate instead of a sixteenth of it, which is what the binary32 instruction has.  f16 has few exponents, so X, A and B are kept times
+// powers of two of each matrix and step: the singular values start below |M| / (|M| + eps), the bound follows them through the
+// polynomial, no entry is larger than the largest singular value, and 2^14 stands for the bound.  hi and lo share a word, so a
+// matrix takes four bytes an element, as in binary32.
 //
-// Every product is written as C[i][j] = sum_k L[i][k] R[j][k] with both operands contiguous in k: X X^T and A A (A is symmetric)
-// are of that form, B X takes X^T, so the product that makes X leaves X^T beside it.  A and B are symmetric: only tiles on or below the
-// diagonal are computed.  Buffers are padded with zeros to whole tiles, which the products reproduce.
+// A and B are symmetric: only tiles on or below the diagonal are computed, and both factors of A = X X^T and A A are read along k.
+// B X reads X by rows of k: its fragments come out of LDS transposed (ds_read_b64_tr_b16).  Buffers are padded with zeros to whole
+// tiles, which the products reproduce.
 #include "pvx_common.h"
 
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-constexpr int kBlk = 256, kBK = 32, kMaxMats = 64, kNormBlocks = 64, kNormChunk = 16384;
+constexpr int kBlk = 256, kBK = 32, kMaxMats = 64, kNormBlocks = 256, kNormChunk = 8192, kMaxSteps = 64, kWhole = 256;
 
 struct Mat {
     const void* in;
     void* out;
     long long base;                      // byte offset of this matrix's buffers in the workspace
     int m, n, mp, np;                    // m <= n; mp, np padded to tiles
-    int tall, splits;                    // in / out are n x m; parts of the sum of X X^T
+    int tall, parts, parts2;             // in / out are n x m; parts of the sums of X X^T and of A A
 };
 
 struct Table {
@@ -38,18 +44,23 @@ struct Table {
     int count;
 };
 
-// buffers of a matrix, in elements of bf16 from its base: X and X^T twice (read / written by turns), A, B, then the f32 parts of A and
-// the f64 parts of the norm
-template <int P> struct Buf {
-    __bf16* base;
-    size_t px, pa;                       // elements of a plane
-    __device__ Buf(char* ws, const Mat& q) : base(reinterpret_cast<__bf16*>(ws + q.base)), px((size_t)q.mp * q.np), pa((size_t)q.mp * q.mp) {}
-    __device__ __forceinline__ __bf16* x(int turn) const { return base + (size_t)turn * P * px; }
-    __device__ __forceinline__ __bf16* xt(int turn) const { return base + (size_t)(2 + turn) * P * px; }
-    __device__ __forceinline__ __bf16* a() const { return base + 4 * P * px; }
-    __device__ __forceinline__ __bf16* b() const { return a() + P * pa; }
-    __device__ __forceinline__ double* sums() const { return reinterpret_cast<double*>(b() + P * pa); }
-    __device__ __forceinline__ float* part() const { return reinterpret_cast<float*>(sums() + kNormBlocks); }
+// a step's factors: the polynomial's coefficients and the powers of two of what they multiply
+struct Scales { float gram, poly0, poly1, poly2, apply, out; };
+
+// buffers of a matrix: X twice (read and written by turns), A and B as words (hi, lo), the parts of the sums, those of the norm
+struct Buf {
+    unsigned* base;
+    size_t px, pa;
+    __device__ Buf(char* ws, const Mat& q) : base(reinterpret_cast<unsigned*>(ws + q.base)), px((size_t)q.mp * q.np), pa((size_t)q.mp * q.mp) {}
+    __device__ __forceinline__ unsigned* x(int turn) const { return base + (size_t)turn * px; }
+    __device__ __forceinline__ unsigned* a() const { return base + 2 * px; }
+    __device__ __forceinline__ unsigned* b() const { return a() + pa; }
+    __device__ __forceinline__ float* part() const { return reinterpret_cast<float*>(b() + pa); }
+    __device__ __forceinline__ double* sums(const Mat& q, int tile) const {
+        const size_t lower = (size_t)(q.mp / tile) * (q.mp / tile + 1) / 2 * tile * tile;
+        return reinterpret_cast<double*>(part() + lower * max(q.parts, q.parts2));
+    }
+    __device__ __forceinline__ Scales* scales(const Mat& q, int tile) const { return reinterpret_cast<Scales*>(sums(q, tile) + kNormBlocks); }
 };
 
 __device__ __forceinline__ int matrix_of(const Table& t, int block) {
@@ -61,23 +72,48 @@ __device__ __forceinline__ int matrix_of(const Table& t, int block) {
     return lo;
 }
 
-template <int P> __device__ __forceinline__ void split(float v, __bf16 (&s)[P]) {
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-        s[p] = (__bf16)v;
-        v -= (float)s[p];
-    }
+__device__ __forceinline__ unsigned pack(float v) {
+    f16x2 h;
+    h[0] = (_Float16)v;
+    h[1] = (_Float16)(v - (float)h[0]);
+    return __builtin_bit_cast(unsigned, h);
+}
+
+__device__ __forceinline__ float value(unsigned w) {
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    return (float)h[0] + (float)h[1];
+}
+
+// the hi halves and the lo halves of eight words
+__device__ __forceinline__ void halves(u32x4 p, u32x4 q, u32x4& hi, u32x4& lo) {
+    hi[0] = __builtin_amdgcn_perm(p[1], p[0], 0x05040100u);
+    hi[1] = __builtin_amdgcn_perm(p[3], p[2], 0x05040100u);
+    hi[2] = __builtin_amdgcn_perm(q[1], q[0], 0x05040100u);
+    hi[3] = __builtin_amdgcn_perm(q[3], q[2], 0x05040100u);
+    lo[0] = __builtin_amdgcn_perm(p[1], p[0], 0x07060302u);
+    lo[1] = __builtin_amdgcn_perm(p[3], p[2], 0x07060302u);
+    lo[2] = __builtin_amdgcn_perm(q[1], q[0], 0x07060302u);
+    lo[3] = __builtin_amdgcn_perm(q[3], q[2], 0x07060302u);
 }
 
 // ---- |M|_F^2, in parts ---------------------------------------------------------------------------------------------------------
 template <typename E>
-__global__ __launch_bounds__(kBlk) void ns_norm_kernel(Table t, char* ws, int planes) {
+__global__ __launch_bounds__(kBlk) void ns_norm_kernel(Table t, char* ws, int tile) {
+    constexpr int V = 16 / (int)sizeof(E);
+    struct alignas(16) Pack { E e[V]; };
     const int id = matrix_of(t, blockIdx.x), k = blockIdx.x - t.first[id], blocks = t.first[id + 1] - t.first[id];
     const Mat& q = t.mat[id];
     const size_t count = (size_t)q.m * q.n;
     const E* in = reinterpret_cast<const E*>(q.in);
+    const size_t packs = (reinterpret_cast<uintptr_t>(in) & 15) == 0 ? count / V : 0;
     double s = 0.0;
-    for (size_t i = (size_t)k * kBlk + threadIdx.x; i < count; i += (size_t)blocks * kBlk) {
+#pragma unroll 4
+    for (size_t i = (size_t)k * kBlk + threadIdx.x; i < packs; i += (size_t)blocks * kBlk) {
+        const Pack p = reinterpret_cast<const Pack*>(in)[i];
+#pragma unroll
+        for (int j = 0; j < V; j++) { const double v = (double)(float)p.e[j]; s = fma(v, v, s); }
+    }
+    for (size_t i = packs * V + (size_t)k * kBlk + threadIdx.x; i < count; i += (size_t)blocks * kBlk) {
         const double v = (double)(float)in[i];
         s = fma(v, v, s);
     }
@@ -86,53 +122,105 @@ __global__ __launch_bounds__(kBlk) void ns_norm_kernel(Table t, char* ws, int pl
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double* sums = planes == 3 ? Buf<3>(ws, q).sums() : Buf<2>(ws, q).sums();
-        sums[k] = red[0] + red[1] + red[2] + red[3];
-        if (k == 0) for (int i = blocks; i < kNormBlocks; i++) sums[i] = 0.0;
+    double* sums = Buf(ws, q).sums(q, tile);
+    if (threadIdx.x == 0) sums[k] = red[0] + red[1] + red[2] + red[3];
+    if (k == 0 && (int)threadIdx.x >= blocks && threadIdx.x < kNormBlocks) sums[threadIdx.x] = 0.0;
+}
+
+// ---- the powers of two ----------------------------------------------------------------------------------------------------------
+// the largest |f| on [0, r] of f(x) = x (a + b x^2 + c x^4) (odd) or a + b x + c x^2: its ends and the roots of its derivative
+__device__ double largest(double a, double b, double c, double r, bool odd) {
+    auto f = [&](double x) { const double y = odd ? x * x : x; return fabs((odd ? x : 1.0) * (a + y * (b + c * y))); };
+    double most = fmax(f(0.0), f(r)), root[2] = {0.0, 0.0};
+    if (!odd) {
+        if (c != 0.0) root[0] = -b / (2.0 * c);
+    } else if (c == 0.0) {                               // a + 3 b y = 0
+        if (b != 0.0) root[0] = -a / (3.0 * b);
+    } else {                                             // a + 3 b y + 5 c y^2 = 0
+        const double d = 9.0 * b * b - 20.0 * a * c;
+        if (d >= 0.0) { root[0] = (-3.0 * b + sqrt(d)) / (10.0 * c); root[1] = (-3.0 * b - sqrt(d)) / (10.0 * c); }
+    }
+    for (int i = 0; i < 2; i++) {
+        const double x = odd ? sqrt(fmax(root[i], 0.0)) : root[i];
+        if (x > 0.0 && x < r) most = fmax(most, f(x));
+    }
+    return most;
+}
+
+// log2 of what a quantity of at most `most` is kept times: 2^14 stands for the next power of two
+__device__ int exponent(double most) {
+    if (!(most > 1e-60)) return most > 0.0 ? 200 : 14;   // (0 and NaN: anything will do)
+    if (!(most < 1e60)) return -200;
+    int e;
+    frexp(most, &e);
+    return 14 - e;
+}
+
+// what X is kept times at the start; its singular values are at most nu = |M| / (|M| + eps)
+__device__ int start_exponent(double nu) { const int e = exponent(1.01 * nu); return e > 120 ? 120 : (e < -80 ? -80 : e); }
+
+__device__ void follow(double nu, int steps, double a, double b, double c, Scales* to) {
+    double r = 1.01 * nu;                                // 1 % a step for what rounding adds
+    int ex = start_exponent(nu);
+    for (int s = 0; s < steps; s++) {
+        const int ea = exponent(1.01 * r * r), eb = exponent(1.01 * largest(a, b, c, 1.01 * r * r, false));
+        r = 1.01 * largest(a, b, c, r, true);
+        int next = exponent(r);
+        next = next > 120 ? 120 : (next < -80 ? -80 : next);
+        Scales k;
+        k.gram = (float)ldexp(1.0, ea - 2 * ex);
+        k.poly0 = (float)ldexp(a, eb);
+        k.poly1 = (float)ldexp(b, eb - ea);
+        k.poly2 = (float)ldexp(c, eb - 2 * ea);
+        k.apply = (float)ldexp(1.0, next - eb - ex);
+        k.out = (float)ldexp(1.0, -eb - ex);
+        to[s] = k;
+        ex = next;
     }
 }
 
-// ---- X and X^T as planes, 32 x 32 elements a workgroup ----------------------------------------------------------------------------
-template <typename E, int P>
-__global__ __launch_bounds__(kBlk) void ns_load_kernel(Table t, char* ws, float eps) {
-    __shared__ float tile[32][33];
-    __shared__ double scale;
-    const int id = matrix_of(t, blockIdx.x);
+// ---- X as words, 64 x 64 elements a workgroup -----------------------------------------------------------------------------------
+template <typename E>
+__global__ __launch_bounds__(kBlk) void ns_load_kernel(Table t, char* ws, int tile, float eps, int steps, float a, float b, float c) {
+    __shared__ float turn[64][65];
+    __shared__ double part[kBlk / 64];
+    const int id = matrix_of(t, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Mat& q = t.mat[id];
-    const Buf<P> buf(ws, q);
-    if (threadIdx.x < 64) {
-        double s = threadIdx.x < kNormBlocks ? buf.sums()[threadIdx.x] : 0.0;
+    const Buf buf(ws, q);
+    static_assert(kNormBlocks == kBlk, "a thread for each part of the norm");
+    double s = buf.sums(q, tile)[threadIdx.x];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
-        if (threadIdx.x == 0) scale = 1.0 / (sqrt(s) + (double)eps);
-    }
-    const int local = blockIdx.x - t.first[id], tn = q.np / 32, i0 = (local / tn) * 32, j0 = (local % tn) * 32;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    const double norm = sqrt(part[0] + part[1] + part[2] + part[3]), nu = norm / (norm + (double)eps);
+    const double scale = ldexp(1.0 / (norm + (double)eps), start_exponent(nu));
+    const int local = blockIdx.x - t.first[id], tn = q.np / 64, i0 = (local / tn) * 64, j0 = (local % tn) * 64;
     const E* in = reinterpret_cast<const E*>(q.in);
-    __syncthreads();
-    for (int r = ty; r < 32; r += 8) {
-        if (!q.tall) {
-            const int i = i0 + r, j = j0 + tx;
-            tile[r][tx] = i < q.m && j < q.n ? (float)((double)(float)in[(size_t)i * q.n + j] * scale) : 0.f;
-        } else {
-            const int j = j0 + r, i = i0 + tx;
-            tile[tx][r] = i < q.m && j < q.n ? (float)((double)(float)in[(size_t)j * q.m + i] * scale) : 0.f;
+    unsigned* x = buf.x(0);
+    if (local == 0 && threadIdx.x == kBlk - 1) {
+        if (steps > 0) follow(nu, steps, a, b, c, buf.scales(q, tile));
+        else buf.scales(q, tile)[0].out = (float)ldexp(1.0, -start_exponent(nu));
+    }
+    if (!q.tall) {
+#pragma unroll 4
+        for (int r = wave; r < 64; r += 4) {
+            const int i = i0 + r, j = j0 + lane;
+            x[(size_t)i * q.np + j] = i < q.m && j < q.n ? pack((float)((double)(float)in[(size_t)i * q.n + j] * scale)) : 0u;
         }
+        return;
+    }
+#pragma unroll 4
+    for (int r = wave; r < 64; r += 4) {
+        const int j = j0 + r, i = i0 + lane;
+        turn[lane][r] = i < q.m && j < q.n ? (float)((double)(float)in[(size_t)j * q.m + i] * scale) : 0.f;
     }
     __syncthreads();
-    for (int r = ty; r < 32; r += 8) {
-        __bf16 s[P];
-        split<P>(tile[r][tx], s);
-#pragma unroll
-        for (int p = 0; p < P; p++) buf.x(0)[p * buf.px + (size_t)(i0 + r) * q.np + j0 + tx] = s[p];
-        split<P>(tile[tx][r], s);
-#pragma unroll
-        for (int p = 0; p < P; p++) buf.xt(0)[p * buf.px + (size_t)(j0 + r) * q.mp + i0 + tx] = s[p];
-    }
+#pragma unroll 4
+    for (int r = wave; r < 64; r += 4) x[(size_t)(i0 + r) * q.np + j0 + lane] = pack(turn[r][lane]);
 }
 
-// ---- the product ------------------------------------------------------------------------------------------------------------------
+// ---- the products ---------------------------------------------------------------------------------------------------------------
 enum { kGram = 0, kPoly = 1, kApply = 2 };
 
 // row and column of tile `l` of the lower triangle
@@ -144,55 +232,57 @@ __device__ __forceinline__ void triangle(int l, int& i, int& j) {
 }
 
 // A workgroup of four waves computes a T x T tile, each wave (T / 2) x (T / 2) in 32 x 32 x 16 instructions.  k goes in steps of 32: the
-// planes of the next step are on their way to registers while this one's are multiplied from LDS.  A row of a step is 64 bytes, four
-// 16-byte pieces; the piece c of row r lies at c ^ (r / 4 mod 4), which spreads sixteen rows over all banks.
-template <typename E, int P, int T, int MODE>
-__global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int cur, int last, float fa, float fb, float fc) {
-    constexpr int Q = T / 64, N = T / 64;                // staging rounds; 32 x 32 blocks of a wave along each side
-    __shared__ u32x4 lds[2][P][T][4];
+// words of the next step are on their way to registers while this one's halves are multiplied from LDS.  Along k a row of a step is 64
+// bytes, four 16-byte pieces, and piece c of row r lies at c ^ (r / 4 mod 4), which spreads sixteen rows over all banks; across k
+// (B X) a row of a step is T columns, 32 bytes apart from the next, so the four rows that a transposing read takes lie in different banks.
+template <typename E, int T, int MODE>
+__global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int step, int last) {
+    constexpr int N = T / 64;                            // staging rounds; 32 x 32 blocks of a wave along each side
+    constexpr int kRow = 2 * T + 32;                     // bytes of a row of k
+    __shared__ u32x4 left[2][T][4];
+    __shared__ __attribute__((aligned(16))) char right[2][MODE == kApply ? kBK * kRow : T * 64];
     const int id = matrix_of(t, blockIdx.x);
     const Mat& q = t.mat[id];
-    const Buf<P> buf(ws, q);
+    const Buf buf(ws, q);
+    const bool whole = q.m <= kWhole;
     int local = blockIdx.x - t.first[id], ti, tj, k0 = 0, k1, part = 0;
-    const __bf16 *L, *R;
-    size_t pl, pr;
-    int ld;
-    if (MODE == kGram) {
-        part = local % q.splits;
-        local /= q.splits;
-        triangle(local, ti, tj);
-        const int steps = PVX_CDIV(q.n, kBK), per = PVX_CDIV(steps, q.splits);
-        k0 = part * per * kBK;
-        k1 = min(steps, (part + 1) * per) * kBK;
-        L = R = buf.x(cur);
-        pl = pr = buf.px;
-        ld = q.np;
-    } else if (MODE == kPoly) {
-        triangle(local, ti, tj);
-        k1 = PVX_CDIV(q.m, kBK) * kBK;
-        L = R = buf.a();
-        pl = pr = buf.pa;
-        ld = q.mp;
-    } else {
+    const unsigned *L, *R;
+    int ld, ldr;
+    if (MODE == kApply) {
         const int tn = q.np / T;
         ti = local / tn;
         tj = local % tn;
         k1 = PVX_CDIV(q.m, kBK) * kBK;
         L = buf.b();
-        R = buf.xt(cur);
-        pl = buf.pa;
-        pr = buf.px;
+        R = buf.x(step & 1);
         ld = q.mp;
+        ldr = q.np;
+    } else {
+        const int parts = MODE == kGram ? q.parts : q.parts2;
+        part = local % parts;
+        local /= parts;
+        triangle(local, ti, tj);
+        const int steps = PVX_CDIV(MODE == kGram ? q.n : q.m, kBK), per = PVX_CDIV(steps, parts);
+        k0 = part * per * kBK;
+        k1 = min(steps, (part + 1) * per) * kBK;
+        L = R = MODE == kGram ? buf.x(step & 1) : buf.a();
+        ld = ldr = MODE == kGram ? q.np : q.mp;
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int srow = tid >> 2, sc = tid & 3;
-    const __bf16* gl = L + (size_t)(ti * T + srow) * ld + sc * 8;
-    const __bf16* gr = R + (size_t)(tj * T + srow) * ld + sc * 8;
-    u32x4 nl[P][Q], nr[P][Q];
-#define NS_FETCH(k)                                                                                                    \
-    _Pragma("unroll") for (int p = 0; p < P; p++) _Pragma("unroll") for (int r = 0; r < Q; r++) {                      \
-        nl[p][r] = *reinterpret_cast<const u32x4*>(gl + p * pl + (size_t)r * 64 * ld + (k));                           \
-        nr[p][r] = *reinterpret_cast<const u32x4*>(gr + p * pr + (size_t)r * 64 * ld + (k));                           \
+    const int srow = tid >> 2, spiece = tid & 3;
+    const unsigned* gl = L + (size_t)(ti * T + srow) * ld + spiece * 8;
+    // across k: 32 rows of T / 8 pieces
+    const int arow = tid / (T / 8), apiece = tid % (T / 8);
+    constexpr int kStride = kBlk / (T / 8);              // rows of k that one round of the workgroup stages
+    const unsigned* gr = MODE == kApply ? R + (size_t)arow * ldr + tj * T + apiece * 8 : R + (size_t)(tj * T + srow) * ldr + spiece * 8;
+    u32x4 nl[N][2], nr[N][2];
+#define NS_FETCH(k)                                                                                                              \
+    _Pragma("unroll") for (int r = 0; r < N; r++) {                                                                              \
+        const u32x4* a__ = reinterpret_cast<const u32x4*>(gl + (size_t)r * 64 * ld + (k));                                       \
+        const u32x4* b__ = reinterpret_cast<const u32x4*>(MODE == kApply ? gr + (size_t)((k) + r * kStride) * ldr                \
+                                                                         : gr + (size_t)r * 64 * ldr + (k));                     \
+        nl[r][0] = a__[0]; nl[r][1] = a__[1];                                                                                    \
+        nr[r][0] = b__[0]; nr[r][1] = b__[1];                                                                                    \
     }
     f32x16 acc[N][N];
 #pragma unroll
@@ -202,149 +292,146 @@ __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
     const int wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2), fr = lane & 31, fh = lane >> 5;
+    // a transposing read: in each group of 16 lanes, lane 4 y + x names row y, columns 4 x .. 4 x + 3 of a block of 4 x 16, and lane c
+    // receives column c of the four rows; groups 0 and 1 take columns 0 .. 31 of k = 0 .. 7, groups 2 and 3 those of k = 8 .. 15
+    const int tr = (8 * fh + ((lane & 15) >> 2)) * kRow + (wj + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
     if (k0 < k1) { NS_FETCH(k0) }
     for (int k = k0; k < k1; k += kBK) {
         __syncthreads();
 #pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int r = 0; r < Q; r++) {
-                const int row = r * 64 + srow, at = sc ^ ((row >> 2) & 3);
-                lds[0][p][row][at] = nl[p][r];
-                lds[1][p][row][at] = nr[p][r];
-            }
+        for (int r = 0; r < N; r++) {
+            const int row = r * 64 + srow, at = spiece ^ ((row >> 2) & 3);
+            u32x4 hi, lo;
+            halves(nl[r][0], nl[r][1], hi, lo);
+            left[0][row][at] = hi;
+            left[1][row][at] = lo;
+            halves(nr[r][0], nr[r][1], hi, lo);
+            const int to = MODE == kApply ? (arow + r * kStride) * kRow + apiece * 16 : row * 64 + at * 16;
+            *reinterpret_cast<u32x4*>(&right[0][to]) = hi;
+            *reinterpret_cast<u32x4*>(&right[1][to]) = lo;
+        }
         __syncthreads();
         if (k + kBK < k1) { NS_FETCH(k + kBK) }
 #pragma unroll
         for (int h = 0; h < kBK / 16; h++) {
-            bf16x8 fl[P][N], fg[P][N];
+            f16x8 fl[2][N], fg[2][N];
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int rl = wi + i * 32 + fr, rr = wj + i * 32 + fr, c = h * 2 + fh;
 #pragma unroll
-                for (int p = 0; p < P; p++) {
-                    fl[p][i] = __builtin_bit_cast(bf16x8, lds[0][p][rl][c ^ ((rl >> 2) & 3)]);
-                    fg[p][i] = __builtin_bit_cast(bf16x8, lds[1][p][rr][c ^ ((rr >> 2) & 3)]);
+                for (int p = 0; p < 2; p++) {
+                    fl[p][i] = __builtin_bit_cast(f16x8, left[p][rl][c ^ ((rl >> 2) & 3)]);
+                    if (MODE == kApply) {
+                        char* at = &right[p][tr + h * 16 * kRow + i * 64];
+                        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+                        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * kRow));
+                        fg[p][i] = __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+                    } else {
+                        fg[p][i] = *reinterpret_cast<const f16x8*>(&right[p][rr * 64 + (c ^ ((rr >> 2) & 3)) * 16]);
+                    }
                 }
             }
+            if (whole) {
 #pragma unroll
-            for (int o = P - 1; o >= 0; o--)             // smallest products first
+                for (int i = 0; i < N; i++)
 #pragma unroll
-                for (int p = 0; p <= o; p++)
+                    for (int j = 0; j < N; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[1][i], fg[1][j], acc[i][j], 0, 0, 0);
+            }
 #pragma unroll
-                    for (int i = 0; i < N; i++)
+            for (int o = 0; o < 3; o++)                  // lo hi, hi lo, hi hi: smallest first
 #pragma unroll
-                        for (int j = 0; j < N; j++)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fl[p][i], fg[o - p][j], acc[i][j], 0, 0, 0);
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < N; j++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[o == 0 ? 1 : 0][i], fg[o == 1 ? 1 : 0][j], acc[i][j], 0, 0, 0);
         }
     }
     // a lane holds column j = lane % 32 and rows 8 g + 4 (lane / 32) + 0 .. 3 of each 32 x 32 block
-    if (MODE == kGram) {
-        const int tiles = (q.mp / T) * (q.mp / T + 1) / 2;
-        float* out = buf.part() + ((size_t)part * tiles + local) * T * T;
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-            for (int j = 0; j < N; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    out[(wi + i * 32 + 8 * (e >> 2) + 4 * fh + (e & 3)) * T + wj + j * 32 + fr] = acc[i][j][e];
-        return;
-    }
-    const __bf16* old = MODE == kPoly ? buf.a() : buf.xt(cur);
-    __bf16* direct = MODE == kPoly ? buf.b() : buf.x(cur ^ 1);
-    __bf16* mirror = MODE == kPoly ? buf.b() : buf.xt(cur ^ 1);
-    const int ldd = MODE == kPoly ? q.mp : q.np;
+    const size_t tiles = (size_t)(q.mp / T) * (q.mp / T + 1) / 2;
+    float* sum = buf.part() + ((size_t)part * tiles + local) * T * T;
+    unsigned* x = buf.x((step & 1) ^ 1);
     E* out = reinterpret_cast<E*>(q.out);
+    float scale = 1.f;
+    if (MODE == kApply) {
+        const Scales& k = buf.scales(q, T)[step];
+        scale = last ? k.out : k.apply;
+    }
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
         for (int j = 0; j < N; j++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int row = ti * T + wi + i * 32 + 8 * g + 4 * fh, col = tj * T + wj + j * 32 + fr;
-                const size_t at = (size_t)col * q.mp + row;      // the old value, read from the mirrored side: four rows at once
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int p = P - 1; p >= 0; p--) {
-                    const bf16x4 o = *reinterpret_cast<const bf16x4*>(old + p * pr + at);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] += (float)o[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = MODE == kPoly ? fb * v[e] + fc * acc[i][j][4 * g + e] : fa * v[e] + acc[i][j][4 * g + e];
-                if (MODE == kApply && last) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (row + e < q.m && col < q.n) out[q.tall ? (size_t)col * q.m + row + e : (size_t)(row + e) * q.n + col] = (E)v[e];
-                    continue;
-                }
-                __bf16 s[4][P];
-#pragma unroll
-                for (int e = 0; e < 4; e++) split<P>(v[e], s[e]);
-#pragma unroll
-                for (int p = 0; p < P; p++) {
-                    bf16x4 o;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        o[e] = s[e][p];
-                        direct[p * pr + (size_t)(row + e) * ldd + col] = s[e][p];
-                    }
-                    if (MODE == kApply || ti != tj) *reinterpret_cast<bf16x4*>(mirror + p * pr + at) = o;
+            for (int e = 0; e < 16; e++) {
+                const int ri = wi + i * 32 + 8 * (e >> 2) + 4 * fh + (e & 3), cj = wj + j * 32 + fr;
+                const float v = acc[i][j][e];
+                if (MODE != kApply) {
+                    sum[ri * T + cj] = v;
+                } else if (last) {
+                    const int row = ti * T + ri, col = tj * T + cj;
+                    if (row < q.m && col < q.n) out[q.tall ? (size_t)col * q.m + row : (size_t)row * q.n + col] = (E)(v * scale);
+                } else {
+                    x[(size_t)(ti * T + ri) * q.np + tj * T + cj] = pack(v * scale);
                 }
             }
 }
 
-// A as planes, both triangles, from the parts of the sum in order; a workgroup takes a 32 x 32 block of a tile
-template <int P, int T>
-__global__ __launch_bounds__(kBlk) void ns_gather_kernel(Table t, char* ws) {
-    __shared__ float tile[32][33];
-    constexpr int kSub = (T / 32) * (T / 32);
+// The parts of a sum of the lower tiles, in order, to words of the whole symmetric matrix: A, or B = a I + b A + c (the sum).  A
+// workgroup takes a 32 x 32 block of a tile, a thread four columns of a row.
+template <int T, int MODE>
+__global__ __launch_bounds__(kBlk) void ns_gather_kernel(Table t, char* ws, int step) {
+    __shared__ unsigned turn[32][33];
+    constexpr int kSide = T / 32;
     const int id = matrix_of(t, blockIdx.x);
     const Mat& q = t.mat[id];
-    const Buf<P> buf(ws, q);
-    const int local = blockIdx.x - t.first[id], l = local / kSub, si = (local % kSub) / (T / 32) * 32, sj = (local % kSub) % (T / 32) * 32;
+    const Buf buf(ws, q);
+    const int local = blockIdx.x - t.first[id], l = local / (kSide * kSide), sub = local % (kSide * kSide);
+    const int si = sub / kSide * 32, sj = sub % kSide * 32;
     int ti, tj;
     triangle(l, ti, tj);
     const size_t tiles = (size_t)(q.mp / T) * (q.mp / T + 1) / 2;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int r = ty; r < 32; r += 8) {
-        float v = 0.f;
-        for (int s = 0; s < q.splits; s++) v += buf.part()[(s * tiles + l) * T * T + (si + r) * T + sj + tx];
-        tile[r][tx] = v;
-        __bf16 o[P];
-        split<P>(v, o);
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4, parts = MODE == kGram ? q.parts : q.parts2;
+    const int row = ti * T + si + r, col = tj * T + sj + c;
+    const f32x4* in = reinterpret_cast<const f32x4*>(buf.part() + (size_t)l * T * T + (si + r) * T + sj + c);
+    const size_t apart = tiles * T * T / 4;
+    const Scales sc = buf.scales(q, T)[step];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < parts; s++) v += in[s * apart];
+    if (MODE == kGram) {
+        v *= sc.gram;
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(buf.a() + (size_t)row * q.mp + col);
 #pragma unroll
-        for (int p = 0; p < P; p++) buf.a()[p * buf.pa + (size_t)(ti * T + si + r) * q.mp + tj * T + sj + tx] = o[p];
+        for (int e = 0; e < 4; e++) v[e] = sc.poly2 * v[e] + sc.poly1 * value(w[e]) + (row == col + e ? sc.poly0 : 0.f);
     }
-    if (ti == tj) return;                                // the diagonal tile is whole already
+    unsigned* to = MODE == kGram ? buf.a() : buf.b();
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = pack(v[e]);
+    *reinterpret_cast<u32x4*>(to + (size_t)row * q.mp + col) = o;
+    if (ti == tj) return;                                // a diagonal tile is whole already
+#pragma unroll
+    for (int e = 0; e < 4; e++) turn[c + e][r] = o[e];
     __syncthreads();
-    for (int r = ty; r < 32; r += 8) {
-        __bf16 o[P];
-        split<P>(tile[tx][r], o);
 #pragma unroll
-        for (int p = 0; p < P; p++) buf.a()[p * buf.pa + (size_t)(tj * T + sj + r) * q.mp + ti * T + si + tx] = o[p];
-    }
+    for (int e = 0; e < 4; e++) o[e] = turn[r][c + e];
+    *reinterpret_cast<u32x4*>(to + (size_t)(tj * T + sj + r) * q.mp + ti * T + si + c) = o;
 }
 
 // steps == 0: the scaled matrix itself
-template <typename E, int P>
-__global__ __launch_bounds__(kBlk) void ns_store_kernel(Table t, char* ws) {
+template <typename E>
+__global__ __launch_bounds__(kBlk) void ns_store_kernel(Table t, char* ws, int tile) {
     const int id = matrix_of(t, blockIdx.x);
     const Mat& q = t.mat[id];
-    const Buf<P> buf(ws, q);
+    const Buf buf(ws, q);
     const size_t i = (size_t)(blockIdx.x - t.first[id]) * kBlk + threadIdx.x;
     if (i >= (size_t)q.m * q.n) return;
     const int w = q.tall ? q.m : q.n;
     const size_t r = i / w, c = i % w;
-    float v = 0.f;
-    for (int p = P - 1; p >= 0; p--) v += (float)(q.tall ? buf.xt(0)[p * buf.px + r * q.mp + c] : buf.x(0)[p * buf.px + r * q.np + c]);
-    reinterpret_cast<E*>(q.out)[i] = (E)v;
+    reinterpret_cast<E*>(q.out)[i] = (E)(value(buf.x(0)[q.tall ? c * q.np + r : r * q.np + c]) * buf.scales(q, tile)[0].out);
 }
 
 int round_up(int v, int to) { return PVX_CDIV(v, to) * to; }
-
-int planes_of(int dtype) { return dtype == PVX_F32 ? 3 : 2; }
 
 // 128 x 128 tiles where the largest product has enough of them for the chip, 64 x 64 otherwise
 int tile_of(const pvx_matrix* mats, int count) {
@@ -355,7 +442,12 @@ int tile_of(const pvx_matrix* mats, int count) {
 
 constexpr int kPartWorkgroups = 512;
 
-void fill(Table& t, const pvx_matrix* mats, int count, int tile, int planes, size_t* total) {
+int parts_of(int want, int k) {          // a part keeps at least four steps
+    const int most = PVX_CDIV(PVX_CDIV(k, kBK), 4);
+    return want < most ? want : most;
+}
+
+void fill(Table& t, const pvx_matrix* mats, int count, int tile, size_t* total) {
     t.count = count;
     size_t off = 0;
     long long tiles = 0;
@@ -370,15 +462,16 @@ void fill(Table& t, const pvx_matrix* mats, int count, int tile, int planes, siz
         q.np = round_up(q.n, tile);
         tiles += (long long)(q.mp / tile) * (q.mp / tile + 1) / 2;
     }
-    // the sum over n is cut where the batch has fewer tiles than fill the chip; a part keeps at least four steps
+    // a sum is cut in parts where the batch has fewer tiles than fill the chip
     const int want = (int)PVX_CDIV((long long)kPartWorkgroups, tiles < 1 ? 1 : tiles);
     for (int i = 0; i < count; i++) {
         Mat& q = t.mat[i];
-        const int most = PVX_CDIV(PVX_CDIV(q.n, kBK), 4);
-        q.splits = want < most ? want : most;
+        q.parts = parts_of(want, q.n);
+        q.parts2 = parts_of(want, q.m);
         q.base = (long long)off;
         const size_t px = (size_t)q.mp * q.np, pa = (size_t)q.mp * q.mp, lower = (size_t)(q.mp / tile) * (q.mp / tile + 1) / 2 * tile * tile;
-        off += pvx_align_up((size_t)planes * 2 * (4 * px + 2 * pa) + sizeof(double) * kNormBlocks + sizeof(float) * lower * q.splits, 256);
+        const int parts = q.parts > q.parts2 ? q.parts : q.parts2;
+        off += pvx_align_up(4 * (2 * px + 2 * pa + lower * parts) + sizeof(double) * kNormBlocks + sizeof(Scales) * kMaxSteps, 256);
     }
     *total = off;
 }
@@ -394,9 +487,10 @@ template <typename F> int spread(Table& t, F blocks) {
     return (int)at;
 }
 
-template <typename E, int P, int T>
+template <typename E, int T>
 int run(Table& t, char* ws, int steps, float a, float b, float c, float eps, hipStream_t st) {
     auto lower = [](const Mat& q) { return (long long)(q.mp / T) * (q.mp / T + 1) / 2; };
+    auto blocks32 = [&](const Mat& q) { return lower(q) * (T / 32) * (T / 32); };
 #define NS_LAUNCH(kernel, blocks_of, ...)                                                      \
     do {                                                                                       \
         const int blocks__ = spread(t, blocks_of);                                             \
@@ -404,19 +498,19 @@ int run(Table& t, char* ws, int steps, float a, float b, float c, float eps, hip
         hipLaunchKernelGGL(kernel, dim3(blocks__), dim3(kBlk), 0, st, t, ws, ##__VA_ARGS__);    \
         PVX_CHECK_LAUNCH();                                                                    \
     } while (0)
-    auto norm_blocks = [](const Mat& q) {
-        const long long k = PVX_CDIV((long long)q.m * q.n, (long long)kNormChunk);
-        return k > kNormBlocks ? (long long)kNormBlocks : k;
-    };
-    NS_LAUNCH((ns_norm_kernel<E>), norm_blocks, P);
-    NS_LAUNCH((ns_load_kernel<E, P>), ([](const Mat& q) { return (long long)(q.mp / 32) * (q.np / 32); }), eps);
-    if (steps == 0) NS_LAUNCH((ns_store_kernel<E, P>), ([](const Mat& q) { return PVX_CDIV((long long)q.m * q.n, (long long)kBlk); }));
+    NS_LAUNCH((ns_norm_kernel<E>), ([](const Mat& q) {
+                  const long long k = PVX_CDIV((long long)q.m * q.n, (long long)kNormChunk);
+                  return k > kNormBlocks ? (long long)kNormBlocks : k;
+              }), T);
+    NS_LAUNCH((ns_load_kernel<E>), ([](const Mat& q) { return (long long)(q.mp / 64) * (q.np / 64); }), T, eps, steps, a, b, c);
+    if (steps == 0) NS_LAUNCH((ns_store_kernel<E>), ([](const Mat& q) { return PVX_CDIV((long long)q.m * q.n, (long long)kBlk); }), T);
     for (int s = 0; s < steps; s++) {
-        const int cur = s & 1, last = s == steps - 1;
-        NS_LAUNCH((ns_product_kernel<E, P, T, kGram>), ([&](const Mat& q) { return lower(q) * q.splits; }), cur, last, a, b, c);
-        NS_LAUNCH((ns_gather_kernel<P, T>), ([&](const Mat& q) { return lower(q) * (T / 32) * (T / 32); }));
-        NS_LAUNCH((ns_product_kernel<E, P, T, kPoly>), lower, cur, last, a, b, c);
-        NS_LAUNCH((ns_product_kernel<E, P, T, kApply>), ([](const Mat& q) { return (long long)(q.mp / T) * (q.np / T); }), cur, last, a, b, c);
+        const int last = s == steps - 1;
+        NS_LAUNCH((ns_product_kernel<E, T, kGram>), ([&](const Mat& q) { return lower(q) * q.parts; }), s, last);
+        NS_LAUNCH((ns_gather_kernel<T, kGram>), blocks32, s);
+        NS_LAUNCH((ns_product_kernel<E, T, kPoly>), ([&](const Mat& q) { return lower(q) * q.parts2; }), s, last);
+        NS_LAUNCH((ns_gather_kernel<T, kPoly>), blocks32, s);
+        NS_LAUNCH((ns_product_kernel<E, T, kApply>), ([](const Mat& q) { return (long long)(q.mp / T) * (q.np / T); }), s, last);
     }
     return PVX_OK;
 }
@@ -437,7 +531,7 @@ extern "C" size_t pvx_orthogonalize_workspace_bytes(const pvx_matrix* mats, int 
     if (check_args(mats, count, dtype) != PVX_OK || count == 0) return 256;
     Table t;
     size_t total;
-    fill(t, mats, count, tile_of(mats, count), planes_of(dtype), &total);
+    fill(t, mats, count, tile_of(mats, count), &total);
     return total;
 }
 
@@ -446,17 +540,18 @@ extern "C" int pvx_orthogonalize(const pvx_matrix* mats, int count, int dtype, i
     const int bad = check_args(mats, count, dtype);
     if (bad != PVX_OK) return bad;
     if (steps < 0 || !(eps >= 0.f)) return PVX_ERR_INVALID;
+    if (steps > kMaxSteps) return PVX_ERR_RANGE;
     if (count == 0) return PVX_OK;
     for (int i = 0; i < count; i++)
         if (!mats[i].in || !mats[i].out) return PVX_ERR_INVALID;
     Table t;
     size_t total;
     const int tile = tile_of(mats, count);
-    fill(t, mats, count, tile, planes_of(dtype), &total);
+    fill(t, mats, count, tile, &total);
     if (!workspace || workspace_bytes < total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return PVX_ERR_WORKSPACE;
     char* ws = reinterpret_cast<char*>(workspace);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == PVX_F32) return tile == 128 ? run<float, 3, 128>(t, ws, steps, a, b, c, eps, st) : run<float, 3, 64>(t, ws, steps, a, b, c, eps, st);
-    if (dtype == PVX_F16) return tile == 128 ? run<_Float16, 2, 128>(t, ws, steps, a, b, c, eps, st) : run<_Float16, 2, 64>(t, ws, steps, a, b, c, eps, st);
-    return tile == 128 ? run<__bf16, 2, 128>(t, ws, steps, a, b, c, eps, st) : run<__bf16, 2, 64>(t, ws, steps, a, b, c, eps, st);
+    if (dtype == PVX_F32) return tile == 128 ? run<float, 128>(t, ws, steps, a, b, c, eps, st) : run<float, 64>(t, ws, steps, a, b, c, eps, st);
+    if (dtype == PVX_F16) return tile == 128 ? run<_Float16, 128>(t, ws, steps, a, b, c, eps, st) : run<_Float16, 64>(t, ws, steps, a, b, c, eps, st);
+    return tile == 128 ? run<__bf16, 128>(t, ws, steps, a, b, c, eps, st) : run<__bf16, 64>(t, ws, steps, a, b, c, eps, st);
 }

@@ -12,7 +12,7 @@ import torch
 from . import _lib
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # a s + b s^3 + c s^5: steepest at 0 of those that keep (0, 1] within about 0.7 .. 1.2
-MAX_MATRICES = 64                             # PVX_ORTHO_MAX
+MAX_MATRICES, MAX_STEPS = 64, 64              # of one call of the C entry
 
 
 def _launch(mats, outs, steps, coefficients, eps):
@@ -35,16 +35,15 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     X = M / (|M|_F + eps) (with the shorter side first), (a, b, c) = coefficients: the singular vectors of M with singular values near 1.
 
     matrices: a matrix [r, c], a batch of them [B, r, c], or a list or tuple of matrices of any sizes; float32 / float16 / bfloat16, on the
-    GPU.  The result has the same form, in the inputs' dtypes: binary32 matrices are computed in binary32 accuracy, 16-bit ones a little
-    above their own.  No gradient flows through it.  Matrices of one dtype go through the GPU together, up to 64 in a call."""
+    GPU.  The result has the same form, in the inputs' dtypes; whatever they are, the products are as accurate as binary32's.  No gradient flows through it.  Matrices of one dtype go through the GPU together, up to 64 in a call."""
     one = isinstance(matrices, torch.Tensor)
     if one and matrices.dim() not in (2, 3):
         raise ValueError("a matrix [r, c] or a batch [B, r, c] is wanted, got %s" % (tuple(matrices.shape),))
     if len(coefficients) != 3:
         raise ValueError("three coefficients are wanted, got %d" % len(coefficients))
     steps, eps, coefficients = int(steps), float(eps), tuple(float(v) for v in coefficients)
-    if steps < 0 or not eps >= 0.0:
-        raise ValueError("steps and eps must not be negative, got %r and %r" % (steps, eps))
+    if not 0 <= steps <= MAX_STEPS or not eps >= 0.0:
+        raise ValueError("steps must be 0 .. %d and eps not negative, got %r and %r" % (MAX_STEPS, steps, eps))
     with torch.no_grad():
         mats = list(matrices.detach().contiguous().unbind(0)) if one and matrices.dim() == 3 else [matrices] if one else list(matrices)
         groups, outs = {}, []
@@ -80,8 +79,8 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
             raise ValueError("lr and weight_decay must not be negative and momentum must be in [0, 1): got %r, %r, %r" % (lr, weight_decay, momentum))
-        if int(steps) < 0 or not eps >= 0.0 or len(coefficients) != 3:
-            raise ValueError("steps and eps must not be negative, with three coefficients: got %r, %r, %r" % (steps, eps, coefficients))
+        if not 0 <= int(steps) <= MAX_STEPS or not eps >= 0.0 or len(coefficients) != 3:
+            raise ValueError("steps must be 0 .. %d and eps not negative, with three coefficients: got %r, %r, %r" % (MAX_STEPS, steps, eps, coefficients))
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps),
                                       coefficients=tuple(coefficients), eps=eps))
 
