@@ -431,6 +431,133 @@ __global__ __launch_bounds__(kBlk) void ns_store_kernel(Table t, char* ws, int t
     reinterpret_cast<E*>(q.out)[i] = (E)(value(buf.x(0)[q.tall ? c * q.np + r : r * q.np + c]) * buf.scales(q, tile)[0].out);
 }
 
+// ---- small matrices: everything in one workgroup ------------------------------------------------------------------------------------
+// X stays in LDS as binary32 and takes the binary32 matrix instruction (16 x 16 x 4): at 16 x 432 the products are nothing and the 27
+// launches of the general form were 96 us.  Rows lie 4 words apart modulo 64, so 16 rows x 4 words touch every bank once.  The sum over
+// k runs in any order, so a lane reads four consecutive k at once and gives one to each of four instructions.
+constexpr int kSmallBlk = 1024, kSmallWaves = kSmallBlk / 64, kSmallWords = 32 * 772;
+constexpr int small_width(int rows) { return (kSmallWords / rows - 4) / 64 * 64; }      // 1536 columns of 16 rows, 768 of 32
+
+template <typename E, int MP>
+__device__ __forceinline__ void small_body(const Mat& q, int steps, float ca, float cb, float cc, float eps, float* x, float* part, float* a, float* b,
+                                           double* red) {
+    constexpr int T = MP / 16, kTiles = T * (T + 1) / 2, kLdA = MP + 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
+    const int m = q.m, n = q.n, np = PVX_CDIV(n, 16) * 16, ld = PVX_CDIV(n, 64) * 64 + 4;
+    const E* in = reinterpret_cast<const E*>(q.in);
+    double s = 0.0;
+    for (int i = tid; i < MP * np; i += kSmallBlk) {
+        const int r = q.tall ? i % MP : i / np, c = q.tall ? i / MP : i % np;
+        float v = 0.f;
+        if (r < m && c < n) v = (float)in[q.tall ? (size_t)c * m + r : (size_t)r * n + c];
+        x[r * ld + c] = v;
+        s = fma((double)v, (double)v, s);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; w++) s += red[w];
+    const double scale = 1.0 / (sqrt(s) + (double)eps);
+    for (int i = tid; i < MP * np; i += kSmallBlk) {
+        const int r = q.tall ? i % MP : i / np, c = q.tall ? i / MP : i % np;
+        x[r * ld + c] = (float)((double)x[r * ld + c] * scale);
+    }
+    for (int step = 0; step < steps; step++) {
+        __syncthreads();
+        f32x4 acc[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = wave * 16; k < np; k += kSmallWaves * 16) {
+            f32x4 f[T];
+#pragma unroll
+            for (int i = 0; i < T; i++) f[i] = *reinterpret_cast<const f32x4*>(&x[(16 * i + lr) * ld + k + 4 * lq]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < T; i++)
+#pragma unroll
+                    for (int j = 0; j <= i; j++)
+                        acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[i][e], f[j][e], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+        }
+        // a lane holds column lane % 16 and rows 4 (lane / 16) + 0 .. 3
+#pragma unroll
+        for (int t = 0; t < kTiles; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[((wave * kTiles + t) * 16 + 4 * lq + e) * 16 + lr] = acc[t][e];
+        __syncthreads();
+        for (int i = tid; i < kTiles * 256; i += kSmallBlk) {
+            const int t = i >> 8, r = (i >> 4) & 15, c = i & 15, ti = t == 0 ? 0 : 1, tj = t == 2 ? 1 : 0;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; w++) v += part[w * kTiles * 256 + i];
+            a[(16 * ti + r) * kLdA + 16 * tj + c] = v;
+            if (ti != tj) a[(16 * tj + c) * kLdA + 16 * ti + r] = v;
+        }
+        __syncthreads();
+        for (int i = tid; i < MP * MP; i += kSmallBlk) {
+            const int r = i / MP, c = i % MP;
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < MP; k++) v = fmaf(a[r * kLdA + k], a[c * kLdA + k], v);
+            b[r * kLdA + c] = fmaf(cc, v, cb * a[r * kLdA + c]);
+        }
+        __syncthreads();
+        // X <- a X + B X by 16 columns, in place: a wave reads all of them before it writes
+        for (int j = wave * 16; j < np; j += kSmallWaves * 16) {
+            f32x4 o[T];
+#pragma unroll
+            for (int i = 0; i < T; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < T; k++) {
+                f32x4 f[T];
+#pragma unroll
+                for (int i = 0; i < T; i++) f[i] = *reinterpret_cast<const f32x4*>(&b[(16 * i + lr) * kLdA + 16 * k + 4 * lq]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float g = x[(16 * k + 4 * lq + e) * ld + j + lr];
+#pragma unroll
+                    for (int i = 0; i < T; i++) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[i][e], g, o[i], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < T; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float* to = &x[(16 * i + 4 * lq + e) * ld + j + lr];
+                    *to = fmaf(ca, *to, o[i][e]);
+                }
+        }
+    }
+    __syncthreads();
+    E* out = reinterpret_cast<E*>(q.out);
+    for (int i = tid; i < m * n; i += kSmallBlk) {
+        const int r = q.tall ? i % m : i / n, c = q.tall ? i / m : i % n;
+        out[i] = (E)x[r * ld + c];
+    }
+}
+
+template <typename E>
+__global__ __launch_bounds__(kSmallBlk) void ns_small_kernel(Table t, int steps, float a, float b, float c, float eps) {
+    __shared__ __attribute__((aligned(16))) float x[kSmallWords];
+    __shared__ __attribute__((aligned(16))) float part[kSmallWaves * 3 * 256];
+    __shared__ __attribute__((aligned(16))) float sa[32 * 36], sb[32 * 36];
+    __shared__ double red[kSmallWaves];
+    const Mat& q = t.mat[blockIdx.x];
+    if (q.m <= 16) small_body<E, 16>(q, steps, a, b, c, eps, x, part, sa, sb, red);
+    else small_body<E, 32>(q, steps, a, b, c, eps, x, part, sa, sb, red);
+}
+
+bool all_small(const pvx_matrix* mats, int count) {
+    for (int i = 0; i < count; i++) {
+        const int m = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols, n = mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows;
+        if (m > 32 || n > small_width(m <= 16 ? 16 : 32)) return false;
+    }
+    return true;
+}
+
 int round_up(int v, int to) { return PVX_CDIV(v, to) * to; }
 
 // 128 x 128 tiles where the largest product has enough of them for the chip, 64 x 64 otherwise
@@ -528,7 +655,7 @@ int check_args(const pvx_matrix* mats, int count, int dtype) {
 }  // namespace
 
 extern "C" size_t pvx_orthogonalize_workspace_bytes(const pvx_matrix* mats, int count, int dtype) {
-    if (check_args(mats, count, dtype) != PVX_OK || count == 0) return 256;
+    if (check_args(mats, count, dtype) != PVX_OK || count == 0 || all_small(mats, count)) return 0;
     Table t;
     size_t total;
     fill(t, mats, count, tile_of(mats, count), &total);
@@ -546,11 +673,18 @@ extern "C" int pvx_orthogonalize(const pvx_matrix* mats, int count, int dtype, i
         if (!mats[i].in || !mats[i].out) return PVX_ERR_INVALID;
     Table t;
     size_t total;
+    hipStream_t st = (hipStream_t)stream;
     const int tile = tile_of(mats, count);
     fill(t, mats, count, tile, &total);
+    if (all_small(mats, count)) {
+        if (dtype == PVX_F32) hipLaunchKernelGGL(ns_small_kernel<float>, dim3(count), dim3(kSmallBlk), 0, st, t, steps, a, b, c, eps);
+        else if (dtype == PVX_F16) hipLaunchKernelGGL(ns_small_kernel<_Float16>, dim3(count), dim3(kSmallBlk), 0, st, t, steps, a, b, c, eps);
+        else hipLaunchKernelGGL(ns_small_kernel<__bf16>, dim3(count), dim3(kSmallBlk), 0, st, t, steps, a, b, c, eps);
+        PVX_CHECK_LAUNCH();
+        return PVX_OK;
+    }
     if (!workspace || workspace_bytes < total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return PVX_ERR_WORKSPACE;
     char* ws = reinterpret_cast<char*>(workspace);
-    hipStream_t st = (hipStream_t)stream;
     if (dtype == PVX_F32) return tile == 128 ? run<float, 128>(t, ws, steps, a, b, c, eps, st) : run<float, 64>(t, ws, steps, a, b, c, eps, st);
     if (dtype == PVX_F16) return tile == 128 ? run<_Float16, 128>(t, ws, steps, a, b, c, eps, st) : run<_Float16, 64>(t, ws, steps, a, b, c, eps, st);
     return tile == 128 ? run<__bf16, 128>(t, ws, steps, a, b, c, eps, st) : run<__bf16, 64>(t, ws, steps, a, b, c, eps, st);

@@ -90,7 +90,7 @@ def test_orthogonalize_codes():
     call = lambda mats, count=None, dtype=0, steps=5, eps=1e-7, ws=P, size=0: L.pvx_orthogonalize(  # noqa: E731
         struct.pack("QQii" * len(mats), *[v for m in mats for v in m]) if mats else None, len(mats) if count is None else count, dtype, steps,
         3.4445, -4.775, 2.0315, eps, ws, size, None)
-    good = (P, P, 16, 432)
+    good = (P, P, 64, 432)
     for args in (dict(mats=[good], count=-1), dict(mats=[], count=2), dict(mats=[good], dtype=3), dict(mats=[good], steps=-1), dict(mats=[good], eps=-1.0),
                  dict(mats=[good], eps=float("nan")), dict(mats=[good, (P, P, 0, 4)]), dict(mats=[(P, P, 4, -1)]), dict(mats=[(0, P, 4, 4)]),
                  dict(mats=[good, (P, 0, 4, 4)])):
@@ -98,8 +98,9 @@ def test_orthogonalize_codes():
     assert call([good] * 65) == RANGE and call([(P, P, 4, (1 << 20) + 1)]) == RANGE
     assert call([]) == 0 and call([good]) == WORKSPACE and call([good], ws=None, size=1 << 30) == WORKSPACE
     need = L.pvx_orthogonalize_workspace_bytes(struct.pack("QQii", *good), 1, 0)
-    assert need > 4 * 16 * 432 and call([good], size=need - 1) == WORKSPACE and call([good], ws=P + 16, size=need) == WORKSPACE
-    assert L.pvx_orthogonalize_workspace_bytes(None, 0, 0) == 256
+    assert need > 4 * 64 * 432 and call([good], size=need - 1) == WORKSPACE and call([good], ws=P + 16, size=need) == WORKSPACE
+    assert L.pvx_orthogonalize_workspace_bytes(None, 0, 0) == 0
+    assert L.pvx_orthogonalize_workspace_bytes(struct.pack("QQii", P, P, 16, 432), 1, 0) == 0     # one workgroup, no workspace
 
 
 def test_optimiser_refuses():
