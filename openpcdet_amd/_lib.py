@@ -55,7 +55,7 @@ SIGNATURES = {
     "pvx_sort_index_workspace_bytes": (c_size_t, [c_int]),
     "pvx_sort_index": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "pvx_lookup_rows_grad_workspace_bytes": (c_size_t, [c_int, c_int]),
-    "pvx_lookup_rows_grad": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+    "pvx_lookup_rows_grad": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
                                      c_size_t, c_void_p]),
     "pvx_group_norm_act_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "pvx_group_norm_act_fwd": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_float,
@@ -198,6 +198,29 @@ def ptr(t):
 def stream(device=None):
     """Raw hipStream_t of PyTorch's current stream (as an integer for ctypes c_void_p)."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """nothing to switch: the tensors' device is the current one"""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *args):
+        return False
+
+
+_HERE_ALREADY = _Here()
+
+
+def on(device):
+    """`with on(tensor.device) as ..`: torch.cuda.device, without its cost where the device is the current one already"""
+    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def raw_stream(device):
+    """the current stream of `device` as ctypes takes it"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def workspace(nbytes, device):

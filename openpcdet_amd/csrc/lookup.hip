@@ -11,8 +11,7 @@
 namespace {
 
 constexpr int kBlk = 256;
-constexpr int kTile = 2048;              // keys of a workgroup in a pass over many tiles
-constexpr int kMaxBits = 11;             // digit of such a pass: 2^22 rows in two passes
+constexpr int kMaxBits = 11;             // digit of a pass over many tiles: 2^22 rows in two passes
 constexpr int kOneBlk = 1024, kOneKeys = 8, kOneMax = kOneBlk * kOneKeys, kOneBits = 8;
 
 template <typename I> __device__ __forceinline__ int key_of(I v, int m) { return v >= 0 && v < (I)m ? (int)v : m; }
@@ -106,73 +105,85 @@ __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__
 }
 
 // ---- many workgroups: per pass a histogram of each tile, a scan along the tiles of each digit, a stable scatter ------------------
-// keys of the first pass come from `index`; those of the later ones from the pass before
-template <typename I>
-__global__ __launch_bounds__(kBlk) void sort_count_kernel(const I* __restrict__ index, int first, int n, int m, int shift, int bits, int tiles,
+// The first pass takes its keys from `index`; between passes key and position travel as one word, the last pass writes them apart.
+template <typename I> struct From {      // the caller's index
+    __device__ static __forceinline__ int key(const I* p, int i, int m) { return key_of<I>(p[i], m); }
+    __device__ static __forceinline__ int2 both(const I* p, int i, int m) { return make_int2(key_of<I>(p[i], m), i); }
+};
+template <> struct From<int2> {
+    __device__ static __forceinline__ int key(const int2* p, int i, int) { return p[i].x; }
+    __device__ static __forceinline__ int2 both(const int2* p, int i, int) { return p[i]; }
+};
+
+// hist[tile * by_tile + digit * by_digit]
+template <typename I, int R>
+__global__ __launch_bounds__(kBlk) void sort_count_kernel(const I* __restrict__ in, int n, int m, int shift, int bits, int by_tile, int by_digit,
                                                           int* __restrict__ hist) {
     extern __shared__ int count[];
     const int digits = 1 << bits;
     for (int d = threadIdx.x; d < digits; d += kBlk) count[d] = 0;
     __syncthreads();
-    const int base = blockIdx.x * kTile;
+    const int base = blockIdx.x * R * kBlk;
 #pragma unroll
-    for (int r = 0; r < kTile / kBlk; r++) {
+    for (int r = 0; r < R; r++) {
         const int i = base + r * kBlk + threadIdx.x;
-        if (i < n) {
-            const I v = index[i];
-            const int key = first ? key_of<I>(v, m) : (int)v;
-            atomicAdd(&count[(key >> shift) & (digits - 1)], 1);
-        }
+        if (i < n) atomicAdd(&count[(From<I>::key(in, i, m) >> shift) & (digits - 1)], 1);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += kBlk) hist[(size_t)d * tiles + blockIdx.x] = count[d];
+    for (int d = threadIdx.x; d < digits; d += kBlk) hist[(size_t)blockIdx.x * by_tile + (size_t)d * by_digit] = count[d];
 }
 
-// a wave for each digit: exclusive scan along its tiles, the digit's total behind them
+// many tiles: a wave for each digit, exclusive scan along its tiles, four at a time for each lane, the digit's total behind them
 __global__ __launch_bounds__(64) void sort_scan_kernel(int* __restrict__ hist, int tiles, int* __restrict__ totals) {
     int* row = hist + (size_t)blockIdx.x * tiles;
+    const int lane = threadIdx.x;
     int carry = 0;
-    for (int base = 0; base < tiles; base += 64) {
-        const int i = base + threadIdx.x;
-        const int v = i < tiles ? row[i] : 0;
-        int incl = v;
+    for (int base = 0; base < tiles; base += 256) {
+        int v[4], sum = 0;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(incl, off); if ((int)threadIdx.x >= off) incl += t; }
-        if (i < tiles) row[i] = carry + incl - v;
+        for (int e = 0; e < 4; e++) {
+            const int i = base + lane * 4 + e;
+            v[e] = i < tiles ? row[i] : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) { const int t = v[e]; v[e] = sum; sum += t; }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(incl, off); if (lane >= off) incl += t; }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = base + lane * 4 + e;
+            if (i < tiles) row[i] = carry + incl - sum + v[e];
+        }
         carry += __shfl(incl, 63);
     }
-    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+    if (lane == 0) totals[blockIdx.x] = carry;
 }
 
-template <typename I>
-__global__ __launch_bounds__(kBlk) void sort_scatter_kernel(const I* __restrict__ index, const int* __restrict__ idx_in, int first, int n, int m,
-                                                            int shift, int bits, int tiles, const int* __restrict__ hist,
-                                                            const int* __restrict__ totals, int* __restrict__ keys_out,
-                                                            int* __restrict__ idx_out) {
-    constexpr int kWaves = kBlk / 64, kRounds = kTile / kBlk;
+// totals: what sort_scan_kernel left, or NULL: hist holds the tiles' own counts, [tile][digit], and this workgroup adds them up itself
+template <typename I, int R, bool LAST>
+__global__ __launch_bounds__(kBlk) void sort_scatter_kernel(const I* __restrict__ in, int n, int m, int shift, int bits, int tiles,
+                                                            const int* __restrict__ hist, const int* __restrict__ totals, int2* __restrict__ out,
+                                                            int* __restrict__ keys, int* __restrict__ order) {
+    constexpr int kWaves = kBlk / 64;
     extern __shared__ int cnt[];                             // [kWaves][digits], then kWaves sums
     const int digits = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int* wsum = cnt + kWaves * digits;
     for (int i = threadIdx.x; i < kWaves * digits; i += kBlk) cnt[i] = 0;
     __syncthreads();
-    const int base = blockIdx.x * kTile + wave * (kTile / kWaves);
-    int key[kRounds], at[kRounds], idx[kRounds];
+    const int base = (blockIdx.x * kWaves + wave) * R * 64;
+    int2 item[R];
+    int at[R];
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) {
+    for (int r = 0; r < R; r++) {
         const int i = base + r * 64 + lane;
-        key[r] = m;
-        idx[r] = i;
-        if (i < n) {
-            const I v = index[i];
-            key[r] = first ? key_of<I>(v, m) : (int)v;
-            if (!first) idx[r] = idx_in[i];
-        }
+        item[r] = i < n ? From<I>::both(in, i, m) : make_int2(m, 0);
     }
     int* mine = cnt + wave * digits;
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) {
+    for (int r = 0; r < R; r++) {
         const bool on = base + r * 64 + lane < n;
-        const int d = (key[r] >> shift) & (digits - 1);
+        const int d = (item[r].x >> shift) & (digits - 1);
         const unsigned long long mask = same_digit(d, bits, on);
         const int before = __popcll(mask & ((1ull << lane) - 1ull));
         at[r] = on ? mine[d] + before : 0;
@@ -181,11 +192,28 @@ __global__ __launch_bounds__(kBlk) void sort_scatter_kernel(const I* __restrict_
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    // where this tile's keys of a digit begin: the digits before it (all tiles), the tiles before this one, the waves before
-    const int per = digits / kBlk > 0 ? digits / kBlk : 1;
-    const int d0 = threadIdx.x * per;
-    int sum = 0;
-    if (d0 < digits) for (int k = 0; k < per; k++) sum += totals[d0 + k];
+    // where this tile's keys of a digit begin: the digits before it (all tiles), the tiles before this one, the waves before.  A thread
+    // takes the digits threadIdx.x * per ..
+    constexpr int kPer = (1 << kMaxBits) / kBlk;
+    const int per = digits / kBlk > 0 ? digits / kBlk : 1, d0 = threadIdx.x * per;
+    int all[kPer], before[kPer], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+        all[k] = before[k] = 0;
+        if (k >= per || d0 + k >= digits) continue;
+        if (totals) {
+            all[k] = totals[d0 + k];
+            before[k] = hist[(size_t)(d0 + k) * tiles + blockIdx.x];
+        } else {
+#pragma unroll 8
+            for (int t = 0; t < tiles; t++) {
+                const int v = hist[(size_t)t * digits + d0 + k];
+                all[k] += v;
+                before[k] += t < (int)blockIdx.x ? v : 0;
+            }
+        }
+        sum += all[k];
+    }
     int incl = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) { const int v = __shfl_up(incl, off); if (lane >= off) incl += v; }
@@ -193,20 +221,20 @@ __global__ __launch_bounds__(kBlk) void sort_scatter_kernel(const I* __restrict_
     __syncthreads();
     int begin = incl - sum;
     for (int w = 0; w < wave; w++) begin += wsum[w];
-    if (d0 < digits) {
-        for (int k = 0; k < per; k++) {
-            int from = begin + hist[(size_t)(d0 + k) * tiles + blockIdx.x];
-            begin += totals[d0 + k];
-            for (int w = 0; w < kWaves; w++) { const int v = cnt[w * digits + d0 + k]; cnt[w * digits + d0 + k] = from; from += v; }
-        }
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+        if (k >= per || d0 + k >= digits) continue;
+        int from = begin + before[k];
+        begin += all[k];
+        for (int w = 0; w < kWaves; w++) { const int v = cnt[w * digits + d0 + k]; cnt[w * digits + d0 + k] = from; from += v; }
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) {
+    for (int r = 0; r < R; r++) {
         if (base + r * 64 + lane < n) {
-            const int to = mine[(key[r] >> shift) & (digits - 1)] + at[r];
-            keys_out[to] = key[r];
-            idx_out[to] = idx[r];
+            const int to = mine[(item[r].x >> shift) & (digits - 1)] + at[r];
+            if (LAST) { keys[to] = item[r].x; order[to] = item[r].y; }
+            else out[to] = item[r];
         }
     }
 }
@@ -228,119 +256,211 @@ __global__ __launch_bounds__(kBlk) void fill_int_kernel(int* __restrict__ p, lon
 // ---- rows ---------------------------------------------------------------------------------------------------------------------
 template <typename E, int V> struct alignas(sizeof(E) * V) Pack { E e[V]; };
 
+// Which row and chunk a thread owns: whole rows side by side in a workgroup, so nothing is divided per element (a 64-bit division a
+// thread was half of the lookup's time); rows wider than a workgroup are walked.
+struct Lane {
+    int slot, chunk, slots;              // row within the workgroup's, first chunk, rows of a workgroup (0: this thread has none)
+    __device__ __forceinline__ explicit Lane(int ch) {
+        const int tw = ch < kBlk ? ch : kBlk;
+        slots = kBlk / tw;
+        slot = threadIdx.x / tw;
+        chunk = slot < slots ? threadIdx.x % tw : ch;
+    }
+    __device__ __forceinline__ long long first() const { return (long long)blockIdx.x * slots + slot; }
+    __device__ __forceinline__ long long step() const { return (long long)gridDim.x * slots; }
+};
+
 template <typename E, int V, typename I>
-__global__ __launch_bounds__(kBlk) void lookup_kernel(const E* __restrict__ table, const I* __restrict__ index, long long chunks, int ch, int m,
-                                                      float scale, E* __restrict__ out) {
+__global__ __launch_bounds__(kBlk) void lookup_kernel(const E* __restrict__ table, const I* __restrict__ index, int n, int ch, int m, float scale,
+                                                      E* __restrict__ out) {
     typedef Pack<E, V> P;
-    for (long long i = (long long)blockIdx.x * kBlk + threadIdx.x; i < chunks; i += (long long)gridDim.x * kBlk) {
-        const long long row = i / ch;
-        const int k = (int)(i - row * ch);
-        const I v = index[row];
-        P p;
-        if (v >= 0 && v < (I)m) {
-            p = reinterpret_cast<const P*>(table)[(long long)v * ch + k];
-            if (scale != 1.f) {
+    constexpr int U = 4;                 // rows on their way together
+    const Lane t(ch);
+    for (int k = t.chunk; k < ch; k += kBlk) {
+        for (long long i = t.first(); i < n; i += U * t.step()) {
+            I v[U];
+            P p[U];
 #pragma unroll
-                for (int j = 0; j < V; j++) p.e[j] = (E)((float)p.e[j] * scale);
+            for (int u = 0; u < U; u++) v[u] = index[min(i + u * t.step(), (long long)n - 1)];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (v[u] >= 0 && v[u] < (I)m) p[u] = reinterpret_cast<const P*>(table)[(long long)v[u] * ch + k];
+                else {
+#pragma unroll
+                    for (int j = 0; j < V; j++) p[u].e[j] = (E)0.f;
+                }
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < V; j++) p.e[j] = (E)0.f;
+            for (int u = 0; u < U; u++) {
+                if (i + u * t.step() >= n) break;
+                if (scale != 1.f && v[u] >= 0 && v[u] < (I)m) {
+#pragma unroll
+                    for (int j = 0; j < V; j++) p[u].e[j] = (E)((float)p[u].e[j] * scale);
+                }
+                reinterpret_cast<P*>(out)[(i + u * t.step()) * ch + k] = p[u];
+            }
         }
-        reinterpret_cast<P*>(out)[i] = p;
     }
 }
 
-// Long runs are added up in blocks of kFan positions (level 1), blocks of kFan such blocks (level 2) and once more (level 3), each only
-// where a whole aligned block carries one key; a row then walks ends position by position and the middle by the largest blocks
-// that fit: at most 2 * 3 * kFan + n / kFan^3 steps for a row, whatever share of the list it has.
-constexpr int kFan = 32, kFanLog = 5, kLevels = 3;
+// The gradient's sums.  `ch` lanes take a block of kFan positions of the sorted list and walk it, eight rows on their way at a time: they
+// add rows up while the key stays, and where it changes the table's row is finished.  A run that crosses a border of the block
+// leaves what the block holds of it: the run that comes in from the left (or is the whole block) as the block's head, the one that goes on
+// to the right as its tail.  Blocks of kFan whole heads, and once more, are added up where they carry one key; then the block in which a
+// crossing run begins joins its tail, whole blocks by the largest that fit, and the last head: at most 2 kWorth + n / kFan^3 steps,
+// whatever share of the list the row has.  (A level is made where the one before has kWorth blocks.)  All work is in proportion to
+// the list, so the table is cleared beforehand; a walk through each row's run by its offsets instead took 1.7 times as long where
+// the runs' lengths differ much.
+constexpr int kFan = 64, kFanLog = 6, kLevels = 3, kWorth = 256;
+
+template <typename E, int V> __device__ __forceinline__ void store_row(E* dtable, long long at, const float (&acc)[V], float scale) {
+    Pack<E, V> o;
+#pragma unroll
+    for (int j = 0; j < V; j++) o.e[j] = (E)(acc[j] * scale);
+    reinterpret_cast<Pack<E, V>*>(dtable)[at] = o;
+}
 
 template <typename E, int V>
-__global__ __launch_bounds__(kBlk) void run_first_kernel(const E* __restrict__ dout, const int* __restrict__ order, const int* __restrict__ offsets,
-                                                         const int* __restrict__ keys, int n, int m, int ch, int blocks,
-                                                         float* __restrict__ part) {
-    typedef Pack<E, V> P;
-    const long long t = (long long)blockIdx.x * kBlk + threadIdx.x;
-    const long long blk = t / ch;
-    if (blk >= blocks) return;
-    const int k = (int)(t - blk * ch), p0 = (int)blk * kFan;
-    const int key = keys[p0];
-    if (key >= m || keys[p0 + kFan - 1] != key) return;
-    float acc[V];
+__global__ __launch_bounds__(kBlk) void run_sum_kernel(const E* __restrict__ dout, const int* __restrict__ order, const int* __restrict__ keys, int n,
+                                                       int m, int ch, int blocks, float scale, float* __restrict__ head, float* __restrict__ tail,
+                                                       E* __restrict__ dtable) {
+    constexpr int U = 8;
+    const Lane t(ch);
+    for (int k = t.chunk; k < ch; k += kBlk) {
+        for (long long blk = t.first(); blk < blocks; blk += t.step()) {
+            const int p0 = (int)blk * kFan, p1 = min(p0 + kFan, n);
+            const int left = p0 > 0 ? keys[p0 - 1] : -1, right = p1 < n ? keys[p1] : -1;
+            int key[U + 1], row[U], begin = p0;
+            float acc[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < kFan; i++) {
-        const int row = order[p0 + i];
-        if ((unsigned)row >= (unsigned)n) continue;
-        const P p = reinterpret_cast<const P*>(dout)[(long long)row * ch + k];
+            for (int j = 0; j < V; j++) acc[j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; j++) acc[j] += (float)p.e[j];
+            for (int u = 0; u < U; u++) {
+                key[u] = keys[min(p0 + u, p1 - 1)];
+                row[u] = order[min(p0 + u, p1 - 1)];
+            }
+            for (int p = p0; p < p1; p += U) {
+                Pack<E, V> q[U];
+                int next_key[U], next_row[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) q[u] = reinterpret_cast<const Pack<E, V>*>(dout)[(long long)min((unsigned)row[u], (unsigned)(n - 1)) * ch + k];
+#pragma unroll
+                for (int u = 0; u < U; u++) {                // those of the next eight, behind the rows
+                    next_key[u] = keys[min(p + U + u, p1 - 1)];
+                    next_row[u] = order[min(p + U + u, p1 - 1)];
+                }
+                key[U] = next_key[0];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int at = p + u, v = key[u];
+                    if (at >= p1) break;
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] += (float)q[u].e[j];
+                    const bool last = at == p1 - 1;
+                    if (!last && key[u + 1] == v) continue;
+                    if (v < m) {
+                        const bool from_left = begin == p0 && left == v, to_right = last && right == v;
+                        if (!from_left && !to_right) {
+                            store_row<E, V>(dtable, (long long)v * ch + k, acc, scale);
+                        } else {
+                            float* o = (begin == p0 ? head : tail) + (blk * ch + k) * V;
+#pragma unroll
+                            for (int j = 0; j < V; j++) o[j] = acc[j];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] = 0.f;
+                    begin = at + 1;
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) { key[u] = next_key[u]; row[u] = next_row[u]; }
+            }
+        }
     }
-    float* o = part + (blk * ch + k) * V;
-#pragma unroll
-    for (int j = 0; j < V; j++) o[j] = acc[j];
 }
 
-// a level's blocks from the level before; shift: log2 of the positions of a block of this level
+// a level's whole blocks from the level before; shift: log2 of the positions of a block of this level
 __global__ __launch_bounds__(kBlk) void run_next_kernel(const float* __restrict__ in, const int* __restrict__ keys, int m, int width, int blocks,
                                                         int shift, float* __restrict__ part) {
-    const long long t = (long long)blockIdx.x * kBlk + threadIdx.x;
-    const long long blk = t / width;
-    if (blk >= blocks) return;
-    const int k = (int)(t - blk * width);
-    const long long p0 = blk << shift;
-    const int key = keys[p0];
-    if (key >= m || keys[p0 + (1LL << shift) - 1] != key) return;
-    float acc = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < kFan; i++) acc += in[(blk * kFan + i) * width + k];
-    part[blk * width + k] = acc;
+    const Lane t(width);
+    for (int k = t.chunk; k < width; k += kBlk) {
+        for (long long blk = t.first(); blk < blocks; blk += t.step()) {
+            const long long p0 = blk << shift;
+            const int key = keys[p0];
+            if (key >= m || keys[p0 + (1LL << shift) - 1] != key) continue;
+            float acc = 0.f;
+#pragma unroll 16
+            for (int i = 0; i < kFan; i++) acc += in[(blk * kFan + i) * width + k];
+            part[blk * width + k] = acc;
+        }
+    }
 }
 
-struct Levels { const float* p[kLevels]; int n; };
+// first position in (p, end] whose key is not `key`; keys ascend and keys[p] == key
+__device__ __forceinline__ int run_end(const int* keys, int p, int end, int key) {
+    int step = kFan;
+    while (p < end - step && keys[p + step] == key) { p += step; step <<= 1; }
+    int hi = p < end - step ? p + step : end;
+    while (hi - p > 1) { const int mid = p + ((hi - p) >> 1); if (keys[mid] == key) p = mid; else hi = mid; }
+    return hi;
+}
 
+struct Levels { const float *p[kLevels], *tail; int n; };
+
+// the rows of runs that cross a border, each by the block it begins in
 template <typename E, int V>
-__global__ __launch_bounds__(kBlk) void row_sum_kernel(const E* __restrict__ dout, const int* __restrict__ order, const int* __restrict__ offsets,
-                                                       int n, int m, int ch, Levels lv, float scale, E* __restrict__ dtable) {
-    typedef Pack<E, V> P;
-    const long long total = (long long)m * ch;
-    for (long long t = (long long)blockIdx.x * kBlk + threadIdx.x; t < total; t += (long long)gridDim.x * kBlk) {
-        const int v = (int)(t / ch), k = (int)(t - (long long)v * ch);
-        int p = offsets[v];
-        const int end = min(offsets[v + 1], n);
-        float acc[V];
+__global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ keys, int n, int m, int ch, int blocks, Levels lv, float scale,
+                                                        E* __restrict__ dtable) {
+    const Lane t(ch);
+    for (int k = t.chunk; k < ch; k += kBlk) {
+        for (long long blk = t.first(); blk < blocks - 1; blk += t.step()) {
+            const int p0 = (int)blk * kFan, v = keys[p0 + kFan - 1];
+            if (v >= m || keys[p0 + kFan] != v) continue;
+            const bool whole = keys[p0] == v;
+            if (whole && p0 > 0 && keys[p0 - 1] == v) continue;                  // it began further left
+            const float* q = (whole ? lv.p[0] : lv.tail) + (blk * ch + k) * V;
+            float acc[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) acc[j] = 0.f;
-        p = max(p, 0);
-        while (p < end) {
-            int level = 0;                   // the largest aligned block that fits
-            while (level < lv.n && (p & ((kFan << (kFanLog * level)) - 1)) == 0 && p <= end - (kFan << (kFanLog * level))) level++;
-            if (level > 0) {
-                const int shift = kFanLog * level;
-                const float* q = lv.p[level - 1] + ((long long)(p >> shift) * ch + k) * V;
+            for (int j = 0; j < V; j++) acc[j] = q[j];
+            int p = p0 + kFan;
+            const int end = run_end(keys, p, n, v);
+            while (p < end) {
+                int level = 1;                       // the largest aligned block that fits
+                while (level < lv.n && (p & ((kFan << (kFanLog * level)) - 1)) == 0 && p <= end - (kFan << (kFanLog * level))) level++;
+                // the blocks of this level up to where a larger one may begin (the last, open one of level 1 is a head), eight at a time
+                const int shift = kFanLog * level, b0 = p >> shift;
+                int b1 = level == 1 ? (int)(((long long)end + kFan - 1) >> kFanLog) : end >> shift;
+                if (level < lv.n) b1 = min(b1, (b0 | (kFan - 1)) + 1);
+                q = lv.p[level - 1] + k * V;
+                for (int b = b0; b < b1; b += 8) {
+                    float w[8][V];
 #pragma unroll
-                for (int j = 0; j < V; j++) acc[j] += q[j];
-                p += 1 << shift;
-                continue;
+                    for (int u = 0; u < 8; u++)
+#pragma unroll
+                        for (int j = 0; j < V; j++) w[u][j] = q[(long long)min(b + u, b1 - 1) * ch * V + j];
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+                        if (b + u < b1) {
+#pragma unroll
+                            for (int j = 0; j < V; j++) acc[j] += w[u][j];
+                        }
+                }
+                if (level == 1 && b1 == (int)(((long long)end + kFan - 1) >> kFanLog)) break;
+                p = b1 << shift;
             }
-            // positions up to the next place a block may begin
-            const int stop = lv.n > 0 ? min(end, (p | (kFan - 1)) + 1) : end;
-#pragma unroll 4
-            for (; p < stop; p++) {
-                const int row = order[p];
-                if ((unsigned)row >= (unsigned)n) continue;
-                const P q = reinterpret_cast<const P*>(dout)[(long long)row * ch + k];
-#pragma unroll
-                for (int j = 0; j < V; j++) acc[j] += (float)q.e[j];
-            }
+            store_row<E, V>(dtable, (long long)v * ch + k, acc, scale);
         }
-        P o;
-#pragma unroll
-        for (int j = 0; j < V; j++) o.e[j] = (E)(acc[j] * scale);
-        reinterpret_cast<P*>(dtable)[t] = o;
     }
+}
+
+__global__ __launch_bounds__(kBlk) void clear_kernel(char* __restrict__ p, long long bytes) {
+    // whole 16-byte pieces between the ends; the allocation begins anywhere
+    const long long head = min(bytes, (long long)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15)), pieces = (bytes - head) / 16;
+    const long long i0 = (long long)blockIdx.x * kBlk + threadIdx.x, step = (long long)gridDim.x * kBlk;
+    uint4* q = reinterpret_cast<uint4*>(p + head);
+    for (long long i = i0; i < pieces; i += step) q[i] = make_uint4(0, 0, 0, 0);
+    for (long long i = i0; i < head; i += step) p[i] = 0;
+    for (long long i = head + pieces * 16 + i0; i < bytes; i += step) p[i] = 0;
 }
 
 int bits_of(int m) {                     // bits of the keys 0 .. m (m >= 1)
@@ -349,60 +469,71 @@ int bits_of(int m) {                     // bits of the keys 0 .. m (m >= 1)
     return b;
 }
 
-int tiles_of(int n) { return (int)PVX_CDIV((long long)n, (long long)kTile); }
+// keys of a thread in a pass: tiles of 1024 keys while they are few, so that the chip has work; of 2048 where their counts would weigh
+int rounds_of(int n) { return n <= (1 << 19) ? 4 : 8; }
+int tiles_of(int n) { return (int)PVX_CDIV((long long)n, (long long)rounds_of(n) * kBlk); }
 
-struct SortWs { int *keys0, *keys1, *idx0, *hist, *totals; };
+struct SortWs { int2 *even, *odd; int *hist, *totals; };
 
 template <typename C> void carve_sort(C& cv, int n, SortWs* w) {
     const bool many = n > kOneMax;
-    const size_t t = many ? (size_t)tiles_of(n) << kMaxBits : 0;
-    w->keys0 = cv.template take<int>(many ? n : 0);
-    w->keys1 = cv.template take<int>(many ? n : 0);
-    w->idx0 = cv.template take<int>(many ? n : 0);
-    w->hist = cv.template take<int>(t);
+    w->even = cv.template take<int2>(many ? n : 0);
+    w->odd = cv.template take<int2>(many ? n : 0);
+    w->hist = cv.template take<int>(many ? (size_t)tiles_of(n) << kMaxBits : 0);
     w->totals = cv.template take<int>(many ? (size_t)1 << kMaxBits : 0);
+}
+
+constexpr int kOwnScan = 1 << 14;        // counts that every scatter workgroup adds up itself rather than leave them to a launch between
+
+template <typename I>
+int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const SortWs& w, int2* out, int* keys, int* order, hipStream_t st) {
+    const int tiles = tiles_of(n), digits = 1 << bits;
+    const bool own = (long long)tiles * digits <= kOwnScan;
+    const size_t lds = sizeof(int) * ((size_t)digits * (kBlk / 64) + kBlk / 64);
+    const int by_tile = own ? digits : 1, by_digit = own ? 1 : tiles;
+    const int* totals = own ? nullptr : w.totals;
+#define SORT_PASS(R)                                                                                                                             \
+    do {                                                                                                                                         \
+        hipLaunchKernelGGL((sort_count_kernel<I, R>), dim3(tiles), dim3(kBlk), sizeof(int) * digits, st, in, n, m, shift, bits, by_tile,         \
+                           by_digit, w.hist);                                                                                                    \
+        PVX_CHECK_LAUNCH();                                                                                                                      \
+        if (!own) {                                                                                                                              \
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(64), 0, st, w.hist, tiles, w.totals);                                        \
+            PVX_CHECK_LAUNCH();                                                                                                                  \
+        }                                                                                                                                        \
+        if (last)                                                                                                                                \
+            hipLaunchKernelGGL((sort_scatter_kernel<I, R, true>), dim3(tiles), dim3(kBlk), lds, st, in, n, m, shift, bits, tiles, w.hist, totals, \
+                               out, keys, order);                                                                                                \
+        else                                                                                                                                     \
+            hipLaunchKernelGGL((sort_scatter_kernel<I, R, false>), dim3(tiles), dim3(kBlk), lds, st, in, n, m, shift, bits, tiles, w.hist,       \
+                               totals, out, keys, order);                                                                                        \
+        PVX_CHECK_LAUNCH();                                                                                                                      \
+    } while (0)
+    if (rounds_of(n) == 4) SORT_PASS(4);
+    else SORT_PASS(8);
+    return PVX_OK;
 }
 
 template <typename I>
 int sort_impl(const I* index, int n, int m, int* order, int* keys, int* offsets, const SortWs& w, hipStream_t st) {
     const int total_bits = bits_of(m);
     if (n <= kOneMax) {
-        const bool inside = m <= 2 * kOneMax;          // few rows: the same workgroup writes their offsets
+        const bool inside = offsets && m <= 2 * kOneMax;       // few rows: the same workgroup writes their offsets
         hipLaunchKernelGGL((sort_one_kernel<I>), dim3(1), dim3(kOneBlk), 0, st, index, n, m, total_bits, order, keys, inside ? offsets : (int*)nullptr);
         PVX_CHECK_LAUNCH();
         if (inside) return PVX_OK;
     } else {
-        const int passes = PVX_CDIV(total_bits, kMaxBits), tiles = tiles_of(n);
-        int shift = 0;
-        const int *kin = nullptr, *iin = nullptr;
-        for (int p = 0; p < passes; p++) {
-            const int bits = PVX_CDIV(total_bits - shift, passes - p), digits = 1 << bits;
-            const bool last = p == passes - 1;
-            // the last pass ends in the caller's arrays: the buffers alternate backwards from there
-            int* kout = last ? keys : ((passes - p) % 2 == 0 ? w.keys0 : w.keys1);
-            int* iout = (passes - 1 - p) % 2 == 0 ? order : w.idx0;
-            const size_t lds = sizeof(int) * ((size_t)digits * (kBlk / 64) + kBlk / 64);
-            if (p == 0) {
-                hipLaunchKernelGGL((sort_count_kernel<I>), dim3(tiles), dim3(kBlk), sizeof(int) * digits, st, index, 1, n, m, shift, bits, tiles, w.hist);
-                PVX_CHECK_LAUNCH();
-                hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(64), 0, st, w.hist, tiles, w.totals);
-                PVX_CHECK_LAUNCH();
-                hipLaunchKernelGGL((sort_scatter_kernel<I>), dim3(tiles), dim3(kBlk), lds, st, index, (const int*)nullptr, 1, n, m, shift, bits, tiles,
-                                   w.hist, w.totals, kout, iout);
-            } else {
-                hipLaunchKernelGGL((sort_count_kernel<int>), dim3(tiles), dim3(kBlk), sizeof(int) * digits, st, kin, 0, n, m, shift, bits, tiles, w.hist);
-                PVX_CHECK_LAUNCH();
-                hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(64), 0, st, w.hist, tiles, w.totals);
-                PVX_CHECK_LAUNCH();
-                hipLaunchKernelGGL((sort_scatter_kernel<int>), dim3(tiles), dim3(kBlk), lds, st, kin, iin, 0, n, m, shift, bits, tiles, w.hist, w.totals,
-                                   kout, iout);
-            }
-            PVX_CHECK_LAUNCH();
-            kin = kout;
-            iin = iout;
+        const int passes = PVX_CDIV(total_bits, kMaxBits);
+        for (int p = 0, shift = 0; p < passes; p++) {
+            const int bits = PVX_CDIV(total_bits - shift, passes - p);
+            int2 *in = p % 2 ? w.even : w.odd, *out = p % 2 ? w.odd : w.even;
+            const int rc = p == 0 ? sort_pass<I>(index, n, m, shift, bits, p == passes - 1, w, out, keys, order, st)
+                                  : sort_pass<int2>(in, n, m, shift, bits, p == passes - 1, w, out, keys, order, st);
+            if (rc != PVX_OK) return rc;
             shift += bits;
         }
     }
+    if (!offsets) return PVX_OK;
     hipLaunchKernelGGL(sort_offsets_kernel, dim3((unsigned)PVX_CDIV((long long)m + 1, (long long)kBlk)), dim3(kBlk), 0, st, keys, n, m, offsets);
     PVX_CHECK_LAUNCH();
     return PVX_OK;
@@ -417,38 +548,48 @@ int vector_of(int width, int dtype, std::initializer_list<const void*> ptrs) {
     return v;
 }
 
-template <typename C> Levels carve_levels(C& cv, int n, int width, float** out) {
+// level 1 has a block for every begun kFan positions, the others for whole ones
+int blocks_of(int n, int level) { return level == 0 ? PVX_CDIV(n, kFan) : n >> (kFanLog * (level + 1)); }
+
+template <typename C> Levels carve_levels(C& cv, int n, int width, float** out, float** tail) {
     Levels lv;
     lv.n = 0;
     for (int l = 0; l < kLevels; l++) {
-        const int blocks = n >> (kFanLog * (l + 1));
-        out[l] = blocks >= 2 ? cv.template take<float>((size_t)blocks * width) : nullptr;
+        const bool worth = l == 0 ? n > kFan : lv.n == l && blocks_of(n, l - 1) >= kWorth;
+        out[l] = worth ? cv.template take<float>((size_t)blocks_of(n, l) * width) : nullptr;
         lv.p[l] = out[l];
-        if (blocks >= 2) lv.n = l + 1;
+        if (worth) lv.n = l + 1;
     }
+    *tail = lv.n > 0 ? cv.template take<float>((size_t)blocks_of(n, 0) * width) : nullptr;
+    lv.tail = *tail;
     return lv;
 }
 
+// workgroups for `rows` rows of `ch` chunks, `each` of them a thread
+dim3 grid_for(long long rows, int ch, int each) {
+    const long long slots = kBlk / (ch < kBlk ? ch : kBlk), blocks = PVX_CDIV(rows, slots * each);
+    return dim3((unsigned)(blocks < 1 ? 1 : (blocks > 65536 ? 65536 : blocks)));
+}
+
 template <typename E, int V>
-int grad_impl(const E* dout, const int* order, const int* keys, const int* offsets, int n, int m, int width, float scale, E* dtable, float** part,
+int grad_impl(const E* dout, const int* order, const int* keys, int n, int m, int width, float scale, E* dtable, float** part, float* tail,
               const Levels& lv, hipStream_t st) {
     const int ch = width / V;
-    for (int l = 0; l < lv.n; l++) {
-        const int blocks = n >> (kFanLog * (l + 1));
-        if (l == 0) {
-            const long long work = (long long)blocks * ch;
-            hipLaunchKernelGGL((run_first_kernel<E, V>), dim3((unsigned)PVX_CDIV(work, (long long)kBlk)), dim3(kBlk), 0, st, dout, order, offsets, keys, n, m,
-                               ch, blocks, part[0]);
-        } else {
-            const long long work = (long long)blocks * width;
-            hipLaunchKernelGGL(run_next_kernel, dim3((unsigned)PVX_CDIV(work, (long long)kBlk)), dim3(kBlk), 0, st, part[l - 1], keys, m, width, blocks,
-                               kFanLog * (l + 1), part[l]);
-        }
+    const long long bytes = (long long)m * width * sizeof(E), want = PVX_CDIV(bytes, 16LL * kBlk * 4);
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(want > 4096 ? 4096 : want)), dim3(kBlk), 0, st, (char*)dtable, bytes);
+    PVX_CHECK_LAUNCH();
+    if (n == 0) return PVX_OK;
+    const int blocks = blocks_of(n, 0);
+    hipLaunchKernelGGL((run_sum_kernel<E, V>), grid_for(blocks, ch, 1), dim3(kBlk), 0, st, dout, order, keys, n, m, ch, blocks, scale,
+                       part[0], tail, dtable);
+    PVX_CHECK_LAUNCH();
+    if (blocks == 1) return PVX_OK;
+    for (int l = 1; l < lv.n; l++) {
+        hipLaunchKernelGGL(run_next_kernel, grid_for(blocks_of(n, l), width, 1), dim3(kBlk), 0, st, part[l - 1], keys, m, width, blocks_of(n, l),
+                           kFanLog * (l + 1), part[l]);
         PVX_CHECK_LAUNCH();
     }
-    const long long work = PVX_CDIV((long long)m * ch, (long long)kBlk);
-    hipLaunchKernelGGL((row_sum_kernel<E, V>), dim3((unsigned)(work > 65536 ? 65536 : work)), dim3(kBlk), 0, st, dout, order, offsets, n, m, ch, lv, scale,
-                       dtable);
+    hipLaunchKernelGGL((run_join_kernel<E, V>), grid_for(blocks - 1, ch, 1), dim3(kBlk), 0, st, keys, n, m, ch, blocks, lv, scale, dtable);
     PVX_CHECK_LAUNCH();
     return PVX_OK;
 }
@@ -462,19 +603,17 @@ int grad_impl(const E* dout, const int* order, const int* keys, const int* offse
     } while (0)
 
 template <typename E>
-int grad_dispatch(const void* dout, const int* order, const int* keys, const int* offsets, int n, int m, int width, float scale, void* dtable,
-                  float** part, const Levels& lv, int v, hipStream_t st) {
-#define LK_GRAD(E, V) grad_impl<E, V>((const E*)dout, order, keys, offsets, n, m, width, scale, (E*)dtable, part, lv, st)
+int grad_dispatch(const void* dout, const int* order, const int* keys, int n, int m, int width, float scale, void* dtable, float** part, float* tail, const Levels& lv, int v, hipStream_t st) {
+#define LK_GRAD(E, V) grad_impl<E, V>((const E*)dout, order, keys, n, m, width, scale, (E*)dtable, part, tail, lv, st)
     LK_DISPATCH(E, v, LK_GRAD);
 }
 
 template <typename E, int V>
 int lookup_impl(const E* table, const void* index, int index64, int n, int m, int width, float scale, E* out, hipStream_t st) {
     const int ch = width / V;
-    const long long chunks = (long long)n * ch, blocks = PVX_CDIV(chunks, (long long)kBlk);
-    const dim3 grid((unsigned)(blocks > 65536 ? 65536 : blocks));
-    if (index64) hipLaunchKernelGGL((lookup_kernel<E, V, long long>), grid, dim3(kBlk), 0, st, table, (const long long*)index, chunks, ch, m, scale, out);
-    else hipLaunchKernelGGL((lookup_kernel<E, V, int>), grid, dim3(kBlk), 0, st, table, (const int*)index, chunks, ch, m, scale, out);
+    const dim3 grid = grid_for(n, ch, n >= 65536 ? 4 : 1);
+    if (index64) hipLaunchKernelGGL((lookup_kernel<E, V, long long>), grid, dim3(kBlk), 0, st, table, (const long long*)index, n, ch, m, scale, out);
+    else hipLaunchKernelGGL((lookup_kernel<E, V, int>), grid, dim3(kBlk), 0, st, table, (const int*)index, n, ch, m, scale, out);
     PVX_CHECK_LAUNCH();
     return PVX_OK;
 }
@@ -499,15 +638,16 @@ extern "C" size_t pvx_sort_index_workspace_bytes(int n) {
     SizerShim shim;
     SortWs w;
     carve_sort(shim, n, &w);
-    return shim.s.total();
+    return shim.s.total() + 256;
 }
 
 extern "C" int pvx_sort_index(const void* index, int index64, int n, int m, int* order, int* keys, int* offsets, void* workspace,
                               size_t workspace_bytes, void* stream) {
-    if (n < 0 || m <= 0 || !offsets || (n > 0 && (!index || !order || !keys))) return PVX_ERR_INVALID;
+    if (n < 0 || m <= 0 || (n > 0 && (!index || !order || !keys))) return PVX_ERR_INVALID;
     if (n > kMaxRows || m > kMaxRows) return PVX_ERR_RANGE;
     hipStream_t st = (hipStream_t)stream;
     if (n == 0) {
+        if (!offsets) return PVX_OK;
         hipLaunchKernelGGL(fill_int_kernel, dim3((unsigned)PVX_CDIV((long long)m + 1, (long long)kBlk)), dim3(kBlk), 0, st, offsets, (long long)m + 1, 0);
         PVX_CHECK_LAUNCH();
         return PVX_OK;
@@ -536,24 +676,24 @@ extern "C" int pvx_lookup_rows(const void* table, int dtype, const void* index, 
 extern "C" size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width) {
     if (n <= 0 || width <= 0) return 256;
     SizerShim shim;
-    float* part[kLevels];
-    carve_levels(shim, n, width, part);
+    float *part[kLevels], *tail;
+    carve_levels(shim, n, width, part, &tail);
     return shim.s.total() + 256;
 }
 
-extern "C" int pvx_lookup_rows_grad(const void* dout, int dtype, const int* order, const int* keys, const int* offsets, int n, int m, int width,
-                                    float scale, void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int pvx_lookup_rows_grad(const void* dout, int dtype, const int* order, const int* keys, int n, int m, int width, float scale,
+                                    void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
     if (n < 0 || m < 0 || width < 0 || dtype < PVX_F32 || dtype > PVX_BF16) return PVX_ERR_INVALID;
     if (m == 0 || width == 0) return PVX_OK;
-    if (!offsets || !dtable || (n > 0 && (!dout || !order || !keys))) return PVX_ERR_INVALID;
+    if (!dtable || (n > 0 && (!dout || !order || !keys))) return PVX_ERR_INVALID;
     if (n > kMaxRows || m > kMaxRows || width > (1 << 24)) return PVX_ERR_RANGE;
     PvxCarver cv(workspace, workspace_bytes);
-    float* part[kLevels];
-    const Levels lv = carve_levels(cv, n, width, part);
+    float *part[kLevels], *tail;
+    const Levels lv = carve_levels(cv, n, width, part, &tail);
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const int v = vector_of(width, dtype, {dout, dtable});
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == PVX_F32) return grad_dispatch<float>(dout, order, keys, offsets, n, m, width, scale, dtable, part, lv, v, st);
-    if (dtype == PVX_F16) return grad_dispatch<_Float16>(dout, order, keys, offsets, n, m, width, scale, dtable, part, lv, v, st);
-    return grad_dispatch<__bf16>(dout, order, keys, offsets, n, m, width, scale, dtable, part, lv, v, st);
+    if (dtype == PVX_F32) return grad_dispatch<float>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
+    if (dtype == PVX_F16) return grad_dispatch<_Float16>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
+    return grad_dispatch<__bf16>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
 }

@@ -107,26 +107,36 @@ def sort_index(index, num_rows):
     num_rows = int(num_rows)
     if num_rows < 1:
         raise ValueError("num_rows must be at least 1, got %d" % num_rows)
-    index = index.reshape(-1).contiguous()
+    return _sort(index.reshape(-1).contiguous(), num_rows)
+
+
+def _sort(index, num_rows, want_offsets=True):
+    """index [n] contiguous"""
     n, dev = index.shape[0], index.device
     L = _lib.lib()
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         order = torch.empty(n, dtype=torch.int32, device=dev)
         keys = torch.empty(n, dtype=torch.int32, device=dev)
-        offsets = torch.empty(num_rows + 1, dtype=torch.int32, device=dev)
-        ws = _lib.workspace(L.pvx_sort_index_workspace_bytes(n), dev)
-        _lib.check(L.pvx_sort_index(_lib.ptr(index), int(index.dtype == torch.int64), n, num_rows, _lib.ptr(order), _lib.ptr(keys),
-                                    _lib.ptr(offsets), _lib.ptr(ws), ws.numel(), _lib.stream()), "pvx_sort_index")
+        offsets = torch.empty(num_rows + 1, dtype=torch.int32, device=dev) if want_offsets else None
+        size = L.pvx_sort_index_workspace_bytes(n)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        rc = L.pvx_sort_index(index.data_ptr(), index.dtype == torch.int64, n, num_rows, order.data_ptr(), keys.data_ptr(),
+                              offsets.data_ptr() if want_offsets else None, ws.data_ptr(), size, _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "pvx_sort_index")
     return IndexSort(order, keys, offsets, num_rows)
 
 
 def _lookup(table, index, scale):
     """table [m, w] contiguous, index [n] contiguous -> [n, w]"""
     n, (m, w) = index.shape[0], table.shape
-    with torch.cuda.device(table.device):
-        out = torch.empty((n, w), dtype=table.dtype, device=table.device)
-        _lib.check(_lib.lib().pvx_lookup_rows(_lib.ptr(table), _lib.DTYPE_CODE[table.dtype], _lib.ptr(index), int(index.dtype == torch.int64),
-                                              n, m, w, scale, _lib.ptr(out), _lib.stream()), "pvx_lookup_rows")
+    dev = table.device
+    with _lib.on(dev):
+        out = torch.empty((n, w), dtype=table.dtype, device=dev)
+        rc = _lib.lib().pvx_lookup_rows(table.data_ptr(), _lib.DTYPE_CODE[table.dtype], index.data_ptr(), index.dtype == torch.int64, n, m, w, scale,
+                                        out.data_ptr(), _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "pvx_lookup_rows")
     return out
 
 
@@ -146,20 +156,22 @@ class _LookupRows(torch.autograd.Function):
         grad = grad.contiguous()
         dtable = torch.empty((m, w), dtype=grad.dtype, device=dev)
         if m > 0 and w > 0:
-            sort = ctx.sort if ctx.sort is not None else sort_index(index, m)
             L = _lib.lib()
-            with torch.cuda.device(dev):
-                ws = _lib.workspace(L.pvx_lookup_rows_grad_workspace_bytes(n, w), dev)
-                _lib.check(L.pvx_lookup_rows_grad(_lib.ptr(grad), _lib.DTYPE_CODE[grad.dtype], _lib.ptr(sort.order), _lib.ptr(sort.keys),
-                                                  _lib.ptr(sort.offsets), n, m, w, ctx.scale, _lib.ptr(dtable), _lib.ptr(ws), ws.numel(),
-                                                  _lib.stream()), "pvx_lookup_rows_grad")
+            with _lib.on(dev):
+                sort = ctx.sort if ctx.sort is not None else _sort(index, m, want_offsets=False)
+                size = L.pvx_lookup_rows_grad_workspace_bytes(n, w)
+                ws = torch.empty(size, dtype=torch.uint8, device=dev)
+                rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], sort.order.data_ptr(), sort.keys.data_ptr(),
+                                            n, m, w, ctx.scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
+                if rc:
+                    _lib.check(rc, "pvx_lookup_rows_grad")
         return dtable, None, None, None
 
 
 def lookup_rows(table, index, scale=1.0, sort=None):
     """scale * table[index]: table [m, ...] float32 / float16 / bfloat16, index int32 or int64 of any shape -> [*index.shape, ...] in the
     table's dtype.  Entries outside [0, m) give zeros and pass no gradient.  The gradient with respect to the table (and only to it) adds
-    each row's entries in their order, in 32 bits, without atomics.  `sort`: sort_index(index, m) of this very index, where the caller
+    each row's entries in 32 bits and in an order of its own, without atomics.  `sort`: sort_index(index, m) of this very index, where the caller
     has it (the backward sorts otherwise)."""
     if not table.is_cuda:
         raise RuntimeError("rows are looked up on the GPU only (no CPU fallback): got a table on %s" % table.device)
@@ -177,10 +189,10 @@ def lookup_rows(table, index, scale=1.0, sort=None):
     width = 1
     for d in table.shape[1:]:
         width *= d
-    flat = table.reshape(table.shape[0], width).contiguous()
-    idx = index.reshape(-1).contiguous()
+    flat = table.contiguous() if table.dim() == 2 else table.reshape(table.shape[0], width).contiguous()
+    idx = index.contiguous() if index.dim() == 1 else index.reshape(-1).contiguous()
     if torch.is_grad_enabled() and flat.requires_grad:
         out = _LookupRows.apply(flat, idx, float(scale), sort)
     else:
         out = _lookup(flat, idx, float(scale))
-    return out.view(shape)
+    return out if out.shape == shape else out.view(shape)

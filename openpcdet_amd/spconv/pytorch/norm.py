@@ -185,20 +185,26 @@ def act_name(module):
     return None
 
 
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
 def _group_norm_fwd(x, weight, bias, residual, offsets, order, samples, groups, eps, act):
-    """x [n, c] contiguous -> y, mean, rstd"""
+    """x [n, c] contiguous -> y, statistics [2, samples, groups] (mean, 1 / sqrt(var + eps))"""
     L = _lib.lib()
     n, c = x.shape
     dev = x.device
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         y = torch.empty_like(x)
         stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
-        ws = _lib.workspace(L.pvx_group_norm_act_workspace_bytes(n, c, samples, int(offsets is not None), groups), dev)
+        size = L.pvx_group_norm_act_workspace_bytes(n, c, samples, offsets is not None, groups)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         base = stats.data_ptr()
-        _lib.check(L.pvx_group_norm_act_fwd(_lib.ptr(x), n, c, _lib.DTYPE_CODE[x.dtype], samples, _lib.ptr(offsets), _lib.ptr(order), groups,
-                                            _lib.ptr(weight), _lib.ptr(bias), _param_code(weight, bias), eps, _lib.ptr(residual), act,
-                                            _lib.ptr(y), base, base + 4 * samples * groups, _lib.ptr(ws), ws.numel(), _lib.stream()),
-                   "pvx_group_norm_act_fwd")
+        rc = L.pvx_group_norm_act_fwd(x.data_ptr(), n, c, _lib.DTYPE_CODE[x.dtype], samples, _addr(offsets), _addr(order), groups, _addr(weight),
+                                      _addr(bias), _param_code(weight, bias), eps, _addr(residual), act, y.data_ptr(), base,
+                                      base + 4 * samples * groups, ws.data_ptr(), size, _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "pvx_group_norm_act_fwd")
     return y, stats
 
 
@@ -224,18 +230,20 @@ class _GroupNormAct(Function):
         n, c = x.shape
         dev = x.device
         dy = dy.contiguous()
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             dx = torch.empty_like(x)
             dres = torch.empty_like(x) if residual is not None else None
             dw = torch.empty_like(weight) if weight is not None else None
             db = torch.empty_like(bias) if bias is not None else None
-            ws = _lib.workspace(L.pvx_group_norm_act_workspace_bytes(n, c, samples, int(offsets is not None), groups), dev)
+            size = L.pvx_group_norm_act_workspace_bytes(n, c, samples, offsets is not None, groups)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
             base = stats.data_ptr()
-            _lib.check(L.pvx_group_norm_act_bwd(_lib.ptr(dy), _lib.ptr(x), _lib.ptr(residual), n, c, _lib.DTYPE_CODE[x.dtype], samples,
-                                                _lib.ptr(offsets), _lib.ptr(order), groups, _lib.ptr(weight), _lib.ptr(bias),
-                                                _param_code(weight, bias), base, base + 4 * samples * groups, act, _lib.ptr(dx), _lib.ptr(dres),
-                                                _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), ws.numel(), _lib.stream()),
-                       "pvx_group_norm_act_bwd")
+            rc = L.pvx_group_norm_act_bwd(dy.data_ptr(), x.data_ptr(), _addr(residual), n, c, _lib.DTYPE_CODE[x.dtype], samples, _addr(offsets),
+                                          _addr(order), groups, _addr(weight), _addr(bias), _param_code(weight, bias), base,
+                                          base + 4 * samples * groups, act, dx.data_ptr(), _addr(dres), _addr(dw), _addr(db), ws.data_ptr(), size,
+                                          _lib.raw_stream(dev))
+            if rc:
+                _lib.check(rc, "pvx_group_norm_act_bwd")
         return dx, dw, db, dres, None, None, None, None, None, None
 
 
@@ -263,17 +271,19 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, re
         raise ValueError("%d channels do not make %d groups" % (c, num_groups))
     if not eps >= 0.0:
         raise ValueError("eps must not be negative, got %r" % (eps,))
+    dev = x.device
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (c,) or p.device != x.device:
+        if p.dim() != 1 or p.shape[0] != c or p.device != dev:
             raise ValueError("%s must be [%d] on %s, got %s on %s" % (name, c, x.device, tuple(p.shape), p.device))
         if p.dtype not in _lib.DTYPE_CODE or (weight is not None and p.dtype != weight.dtype):
             raise TypeError("weight and bias must share one of float32, float16 and bfloat16, got %s for %s" % (p.dtype, name))
     if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device:
+        if residual.shape != x.shape or residual.device != dev:
             raise ValueError("residual must be %s on %s, got %s on %s" % (tuple(x.shape), x.device, tuple(residual.shape), residual.device))
-        residual = residual.to(x.dtype)
+        if residual.dtype != x.dtype:
+            residual = residual.to(x.dtype)
     if offsets is None:
         if order is not None:
             raise ValueError("order needs offsets")
@@ -281,21 +291,24 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, re
     else:
         if x.dim() != 2:
             raise ValueError("with offsets, x must be [N, C], got %s" % (tuple(x.shape),))
-        for name, t, shape in (("offsets", offsets, None), ("order", order, (x.shape[0],))):
+        for name, t, size in (("offsets", offsets, None), ("order", order, x.shape[0])):
             if t is None:
                 continue
-            if t.dtype != torch.int32 or t.dim() != 1 or t.device != x.device or (shape is not None and tuple(t.shape) != shape):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.device != dev or (size is not None and t.shape[0] != size):
                 raise ValueError("%s must be an int32 vector%s on %s, got %s %s on %s" % (
-                    name, " of %d" % shape if shape else "", x.device, t.dtype, tuple(t.shape), t.device))
+                    name, " of %d" % size if size is not None else "", x.device, t.dtype, tuple(t.shape), t.device))
         samples = offsets.shape[0] - 1
         if samples < 1:
             raise ValueError("offsets must have an entry more than there are samples")
         offsets = offsets.contiguous()
         order = order.contiguous() if order is not None else None
-    flat = x.reshape(-1, c).contiguous()
+    plain = x.dim() == 2
+    flat = x.contiguous() if plain else x.reshape(-1, c).contiguous()
     if flat.shape[0] == 0:
         samples = max(samples, 1)
-    res = residual.reshape(-1, c).contiguous() if residual is not None else None
+    res = residual
+    if res is not None:
+        res = res.contiguous() if plain else res.reshape(-1, c).contiguous()
     w = weight.contiguous() if weight is not None else None
     b = bias.contiguous() if bias is not None else None
     args = (flat, w, b, res, offsets, order, samples, num_groups, eps, _ACTS[act])
@@ -303,7 +316,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, re
         y = _GroupNormAct.apply(*args)
     else:
         y = _group_norm_fwd(*args)[0]
-    return y.view(x.shape)
+    return y if plain else y.view(x.shape)
 
 
 class SparseGroupNorm(SparseModule):

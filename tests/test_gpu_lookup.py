@@ -1,6 +1,8 @@
 """Rows looked up by index and the table's gradient by sorted index (csrc/lookup.hip; scatter.lookup_rows, scatter.sort_index) against
-plain float64 forms.  The forward is one product rounded once.  A gradient row of k entries is a sum in binary32 whose longest chain has
-at most 3 * 2 * 32 + k / 32^3 + 3 * 32 terms, times the scale, rounded once: |error| <= chain * 2^-24 * sum |dout| |scale| + eps / 2 |value|."""
+plain float64 forms.  The forward is one product rounded once.  A gradient row of k entries is a sum in binary32 along a chain of at
+most 3 * 64 additions inside blocks of three levels and, behind them, a head, a tail, 2 * 255 blocks of two levels and k / 64^3 of the
+third: fewer than 828 + k / 64^3 roundings of partial sums no larger than sum |dout|; then the scale and one rounding more:
+|error| <= (828 + k / 64^3 + 1) * 2^-24 * sum |dout| |scale| + eps / 2 |value|."""
 import pytest
 import torch
 
@@ -45,7 +47,7 @@ def check(dev, n, m, w, dtype=torch.float32, itype=torch.int64, kind="uniform", 
     ref = torch.zeros(m, w, dtype=torch.float64, device=dev).index_add_(0, at, d64) * scale32
     mag = torch.zeros(m, w, dtype=torch.float64, device=dev).index_add_(0, at, d64.abs()) * abs(scale32)
     count = torch.bincount(at[inside], minlength=m).double().unsqueeze(1)
-    chain = torch.minimum(count, 288 + count / 32768) + 1
+    chain = torch.minimum(count, 828 + count / 64 ** 3) + 1
     bound = chain * U * mag
     bound = bound + torch.finfo(dtype).eps / 2 * (ref.abs() + bound) + (2.0 ** -25 if dtype == torch.float16 else 0)
     err = (got.double() - ref).abs()
