@@ -541,16 +541,17 @@ int pvx_bn_act_bwd_sync(const void* dy, const void* x, const void* y, int n, int
  *                         end; keys [n] = the sorted indices (m for those outside); offsets [m + 1]: row v's run is
  *                         order[offsets[v]] .. order[offsets[v + 1]] (NULL: not wanted).  m >= 1
  *   pvx_lookup_rows_grad  dtable[v] = scale * sum of dout over row v's run, in binary32 and in a fixed order, rounded once; rows with no
- *                         entry are zero, every row is written.  No atomics: the same result on every run.
+ *                         entry are zero, every row is written.  No atomics: the same result on every run.  order and keys are
+ *                         those of pvx_sort_index (workspace size: sorted = 1), or NULL, and the call sorts `index` itself
  * ---------------------------------------------------------------------------------------------------- */
 int pvx_lookup_rows(const void* table, int dtype, const void* index, int index64, int n, int m, int width, float scale, void* out,
                     void* stream);
 size_t pvx_sort_index_workspace_bytes(int n);
 int pvx_sort_index(const void* index, int index64, int n, int m, int* order, int* keys, int* offsets, void* workspace,
                    size_t workspace_bytes, void* stream);
-size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width);
-int pvx_lookup_rows_grad(const void* dout, int dtype, const int* order, const int* keys, int n, int m, int width, float scale,
-                         void* dtable, void* workspace, size_t workspace_bytes, void* stream);
+size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width, int sorted);
+int pvx_lookup_rows_grad(const void* dout, int dtype, const void* index, int index64, const int* order, const int* keys, int n, int m,
+                         int width, float scale, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ----------------------------------------------------------------------------------------------------
  * Group norm over the rows of a channels-last matrix x [n, c], fused with (+ residual) -> activation: the normalisation for a

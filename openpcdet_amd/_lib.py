@@ -54,8 +54,8 @@ SIGNATURES = {
     "pvx_lookup_rows": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),
     "pvx_sort_index_workspace_bytes": (c_size_t, [c_int]),
     "pvx_sort_index": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "pvx_lookup_rows_grad_workspace_bytes": (c_size_t, [c_int, c_int]),
-    "pvx_lookup_rows_grad": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+    "pvx_lookup_rows_grad_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "pvx_lookup_rows_grad": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
                                      c_size_t, c_void_p]),
     "pvx_group_norm_act_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "pvx_group_norm_act_fwd": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_float,

@@ -673,26 +673,43 @@ extern "C" int pvx_lookup_rows(const void* table, int dtype, const void* index, 
     return lookup_dispatch<__bf16>(table, index, index64, n, m, width, scale, out, v, st);
 }
 
-extern "C" size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width) {
+extern "C" size_t pvx_lookup_rows_grad_workspace_bytes(int n, int width, int sorted) {
     if (n <= 0 || width <= 0) return 256;
     SizerShim shim;
     float *part[kLevels], *tail;
+    SortWs w;
     carve_levels(shim, n, width, part, &tail);
+    if (!sorted) {
+        shim.take<int>(n);
+        shim.take<int>(n);
+        carve_sort(shim, n, &w);
+    }
     return shim.s.total() + 256;
 }
 
-extern "C" int pvx_lookup_rows_grad(const void* dout, int dtype, const int* order, const int* keys, int n, int m, int width, float scale,
-                                    void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int pvx_lookup_rows_grad(const void* dout, int dtype, const void* index, int index64, const int* order, const int* keys, int n, int m,
+                                    int width, float scale, void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
     if (n < 0 || m < 0 || width < 0 || dtype < PVX_F32 || dtype > PVX_BF16) return PVX_ERR_INVALID;
     if (m == 0 || width == 0) return PVX_OK;
-    if (!dtable || (n > 0 && (!dout || !order || !keys))) return PVX_ERR_INVALID;
+    if (!dtable || !order != !keys || (n > 0 && (!dout || (!order && !index)))) return PVX_ERR_INVALID;
     if (n > kMaxRows || m > kMaxRows || width > (1 << 24)) return PVX_ERR_RANGE;
     PvxCarver cv(workspace, workspace_bytes);
     float *part[kLevels], *tail;
     const Levels lv = carve_levels(cv, n, width, part, &tail);
+    hipStream_t st = (hipStream_t)stream;
+    if (!order && n > 0) {
+        int *own = cv.take<int>(n), *own_keys = cv.take<int>(n);
+        SortWs w;
+        carve_sort(cv, n, &w);
+        if (!cv.ok()) return PVX_ERR_WORKSPACE;
+        const int rc = index64 ? sort_impl<long long>((const long long*)index, n, m, own, own_keys, nullptr, w, st)
+                               : sort_impl<int>((const int*)index, n, m, own, own_keys, nullptr, w, st);
+        if (rc != PVX_OK) return rc;
+        order = own;
+        keys = own_keys;
+    }
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const int v = vector_of(width, dtype, {dout, dtable});
-    hipStream_t st = (hipStream_t)stream;
     if (dtype == PVX_F32) return grad_dispatch<float>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
     if (dtype == PVX_F16) return grad_dispatch<_Float16>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
     return grad_dispatch<__bf16>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);

@@ -17,6 +17,8 @@
 // tiles, which the products reproduce.
 #include "pvx_common.h"
 
+#include <math.h>
+
 namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -29,6 +31,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 constexpr int kBlk = 256, kBK = 32, kMaxMats = 64, kNormBlocks = 256, kNormChunk = 8192, kMaxSteps = 64, kWhole = 256;
+
 
 struct Mat {
     const void* in;
@@ -63,13 +66,10 @@ struct Buf {
     __device__ __forceinline__ Scales* scales(const Mat& q, int tile) const { return reinterpret_cast<Scales*>(sums(q, tile) + kNormBlocks); }
 };
 
+// the matrix of a workgroup, in one load of the wave instead of a search's six
 __device__ __forceinline__ int matrix_of(const Table& t, int block) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= block) lo = mid; else hi = mid - 1;
-    }
-    return lo;
+    const int lane = threadIdx.x & 63;
+    return __popcll(__ballot(lane < t.count && t.first[lane + 1] <= block));
 }
 
 __device__ __forceinline__ unsigned pack(float v) {
@@ -128,60 +128,75 @@ __global__ __launch_bounds__(kBlk) void ns_norm_kernel(Table t, char* ws, int ti
 }
 
 // ---- the powers of two ----------------------------------------------------------------------------------------------------------
-// the largest |f| on [0, r] of f(x) = x (a + b x^2 + c x^4) (odd) or a + b x + c x^2: its ends and the roots of its derivative
-__device__ double largest(double a, double b, double c, double r, bool odd) {
-    auto f = [&](double x) { const double y = odd ? x * x : x; return fabs((odd ? x : 1.0) * (a + y * (b + c * y))); };
-    double most = fmax(f(0.0), f(r)), root[2] = {0.0, 0.0};
-    if (!odd) {
-        if (c != 0.0) root[0] = -b / (2.0 * c);
-    } else if (c == 0.0) {                               // a + 3 b y = 0
-        if (b != 0.0) root[0] = -a / (3.0 * b);
-    } else {                                             // a + 3 b y + 5 c y^2 = 0
-        const double d = 9.0 * b * b - 20.0 * a * c;
+// What the singular values' bound r becomes in a step: the largest |f| on [0, r] of f(x) = x (a + b x^2 + c x^4), at its end or at a root
+// of its derivative a + 3 b y + 5 c y^2, y = x^2.  The roots come from the host; binary32 will do: the exponents are bounds, with 1 %
+// and more to spare a step.
+struct Poly {
+    float a, b, c;
+    float x[2], f[2];                    // where |f| may have its extremes, and |f| there; 0 where there is none
+    __device__ __forceinline__ float largest(float r) const {
+        const float y = r * r;
+        float most = fabsf(r * (a + y * (b + y * c)));
+        if (x[0] < r) most = fmaxf(most, f[0]);
+        if (x[1] < r) most = fmaxf(most, f[1]);
+        return most;
+    }
+};
+
+Poly poly_of(float a, float b, float c) {
+    Poly p{a, b, c, {0.f, 0.f}, {0.f, 0.f}};
+    double root[2] = {0.0, 0.0};
+    if (c == 0.f) {
+        if (b != 0.f) root[0] = -(double)a / (3.0 * b);
+    } else {
+        const double d = 9.0 * b * b - 20.0 * (double)a * c;
         if (d >= 0.0) { root[0] = (-3.0 * b + sqrt(d)) / (10.0 * c); root[1] = (-3.0 * b - sqrt(d)) / (10.0 * c); }
     }
     for (int i = 0; i < 2; i++) {
-        const double x = odd ? sqrt(fmax(root[i], 0.0)) : root[i];
-        if (x > 0.0 && x < r) most = fmax(most, f(x));
+        if (!(root[i] > 0.0)) continue;
+        const double x = sqrt(root[i]);
+        p.x[i] = (float)x;
+        p.f[i] = (float)fabs(x * (a + root[i] * (b + root[i] * c)));
     }
-    return most;
+    return p;
 }
 
-// log2 of what a quantity of at most `most` is kept times: 2^14 stands for the next power of two
-__device__ int exponent(double most) {
-    if (!(most > 1e-60)) return most > 0.0 ? 200 : 14;   // (0 and NaN: anything will do)
-    if (!(most < 1e60)) return -200;
-    int e;
-    frexp(most, &e);
-    return 14 - e;
+// the power of two above `most`, within what the scales can hold; 0 and NaN: anything will do
+__device__ __forceinline__ int above(float most) {
+    if (!(most > 1e-30f)) return most > 0.f ? -99 : 0;
+    if (!(most < 1e9f)) return 30;
+    return __builtin_amdgcn_frexp_expf(most);
 }
 
-// what X is kept times at the start; its singular values are at most nu = |M| / (|M| + eps)
-__device__ int start_exponent(double nu) { const int e = exponent(1.01 * nu); return e > 120 ? 120 : (e < -80 ? -80 : e); }
+__device__ __forceinline__ float two(int e) { return ldexpf(1.f, e); }
 
-__device__ void follow(double nu, int steps, double a, double b, double c, Scales* to) {
-    double r = 1.01 * nu;                                // 1 % a step for what rounding adds
-    int ex = start_exponent(nu);
+// X is kept times 2^(14 - above(its largest singular value)); at the start that is below nu = |M| / (|M| + eps)
+__device__ __forceinline__ int start_above(float nu) { return above(1.01f * nu); }
+
+__device__ void follow(float nu, int steps, const Poly& f, Scales* to) {
+    float r = 1.01f * nu;                                // 1 % a step for what rounding adds
+    int er = start_above(nu);
     for (int s = 0; s < steps; s++) {
-        const int ea = exponent(1.01 * r * r), eb = exponent(1.01 * largest(a, b, c, 1.01 * r * r, false));
-        r = 1.01 * largest(a, b, c, r, true);
-        int next = exponent(r);
-        next = next > 120 ? 120 : (next < -80 ? -80 : next);
+        const int ea = 14 - 2 * er;                      // A <= 2^(2 er)
+        const float y = r * r;
+        const int eb = 14 - above(1.01f * (fabsf(f.a) + y * (fabsf(f.b) + y * fabsf(f.c))));
+        r = 1.01f * f.largest(r);
+        const int next = above(r);
         Scales k;
-        k.gram = (float)ldexp(1.0, ea - 2 * ex);
-        k.poly0 = (float)ldexp(a, eb);
-        k.poly1 = (float)ldexp(b, eb - ea);
-        k.poly2 = (float)ldexp(c, eb - 2 * ea);
-        k.apply = (float)ldexp(1.0, next - eb - ex);
-        k.out = (float)ldexp(1.0, -eb - ex);
+        k.gram = two(ea - 2 * (14 - er));
+        k.poly0 = ldexpf(f.a, eb);
+        k.poly1 = ldexpf(f.b, eb - ea);
+        k.poly2 = ldexpf(f.c, eb - 2 * ea);
+        k.apply = two(14 - next - eb - (14 - er));
+        k.out = two(-eb - (14 - er));
         to[s] = k;
-        ex = next;
+        er = next;
     }
 }
 
 // ---- X as words, 64 x 64 elements a workgroup -----------------------------------------------------------------------------------
 template <typename E>
-__global__ __launch_bounds__(kBlk) void ns_load_kernel(Table t, char* ws, int tile, float eps, int steps, float a, float b, float c) {
+__global__ __launch_bounds__(kBlk) void ns_load_kernel(Table t, char* ws, int tile, float eps, int steps, Poly poly) {
     __shared__ float turn[64][65];
     __shared__ double part[kBlk / 64];
     const int id = matrix_of(t, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -193,20 +208,33 @@ __global__ __launch_bounds__(kBlk) void ns_load_kernel(Table t, char* ws, int ti
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
     if (lane == 0) part[wave] = s;
     __syncthreads();
-    const double norm = sqrt(part[0] + part[1] + part[2] + part[3]), nu = norm / (norm + (double)eps);
-    const double scale = ldexp(1.0 / (norm + (double)eps), start_exponent(nu));
+    const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
+    const float nu = (float)(norm / (norm + (double)eps));
+    const double scale = ldexp(1.0 / (norm + (double)eps), 14 - start_above(nu));
     const int local = blockIdx.x - t.first[id], tn = q.np / 64, i0 = (local / tn) * 64, j0 = (local % tn) * 64;
     const E* in = reinterpret_cast<const E*>(q.in);
     unsigned* x = buf.x(0);
     if (local == 0 && threadIdx.x == kBlk - 1) {
-        if (steps > 0) follow(nu, steps, a, b, c, buf.scales(q, tile));
-        else buf.scales(q, tile)[0].out = (float)ldexp(1.0, -start_exponent(nu));
+        if (steps > 0) follow(nu, steps, poly, buf.scales(q, tile));
+        else buf.scales(q, tile)[0].out = two(start_above(nu) - 14);
     }
-    if (!q.tall) {
-#pragma unroll 4
-        for (int r = wave; r < 64; r += 4) {
-            const int i = i0 + r, j = j0 + lane;
-            x[(size_t)i * q.np + j] = i < q.m && j < q.n ? pack((float)((double)(float)in[(size_t)i * q.n + j] * scale)) : 0u;
+    if (!q.tall) {                                       // sixteen lanes a row, four columns each
+        const int j = j0 + 4 * (lane & 15);
+        struct alignas(4 * sizeof(E)) Four { E e[4]; };
+        const bool whole = q.n % 4 == 0 && reinterpret_cast<uintptr_t>(in) % sizeof(Four) == 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int i = i0 + 16 * r + 4 * wave + (lane >> 4);
+            Four f;
+            if (whole && i < q.m && j < q.n) f = *reinterpret_cast<const Four*>(in + (size_t)i * q.n + j);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) f.e[e] = i < q.m && j + e < q.n ? in[(size_t)i * q.n + j + e] : (E)0.f;
+            }
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = pack((float)((double)(float)f.e[e] * scale));
+            *reinterpret_cast<u32x4*>(x + (size_t)i * q.np + j) = o;
         }
         return;
     }
@@ -239,8 +267,9 @@ template <typename E, int T, int MODE>
 __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int step, int last) {
     constexpr int N = T / 64;                            // staging rounds; 32 x 32 blocks of a wave along each side
     constexpr int kRow = 2 * T + 32;                     // bytes of a row of k
-    __shared__ u32x4 left[2][T][4];
-    __shared__ __attribute__((aligned(16))) char right[2][MODE == kApply ? kBK * kRow : T * 64];
+    constexpr int kD = T == 128 ? 1 : 2;                 // buffers: three workgroups of one, four of two on a CU (measured: the better ones)
+    __shared__ u32x4 left[kD][2][T][4];
+    __shared__ __attribute__((aligned(16))) char right[kD][2][MODE == kApply ? kBK * kRow : T * 64];
     const int id = matrix_of(t, blockIdx.x);
     const Mat& q = t.mat[id];
     const Buf buf(ws, q);
@@ -295,23 +324,32 @@ __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int
     // a transposing read: in each group of 16 lanes, lane 4 y + x names row y, columns 4 x .. 4 x + 3 of a block of 4 x 16, and lane c
     // receives column c of the four rows; groups 0 and 1 take columns 0 .. 31 of k = 0 .. 7, groups 2 and 3 those of k = 8 .. 15
     const int tr = (8 * fh + ((lane & 15) >> 2)) * kRow + (wj + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#define NS_STAGE(d)                                                                                                              \
+    _Pragma("unroll") for (int r = 0; r < N; r++) {                                                                              \
+        const int row = r * 64 + srow, at = spiece ^ ((row >> 2) & 3);                                                           \
+        u32x4 hi, lo;                                                                                                            \
+        halves(nl[r][0], nl[r][1], hi, lo);                                                                                      \
+        left[d][0][row][at] = hi;                                                                                                \
+        left[d][1][row][at] = lo;                                                                                                \
+        halves(nr[r][0], nr[r][1], hi, lo);                                                                                      \
+        const int to = MODE == kApply ? (arow + r * kStride) * kRow + apiece * 16 : row * 64 + at * 16;                          \
+        *reinterpret_cast<u32x4*>(&right[d][0][to]) = hi;                                                                        \
+        *reinterpret_cast<u32x4*>(&right[d][1][to]) = lo;                                                                        \
+    }
     if (k0 < k1) { NS_FETCH(k0) }
+    if (kD == 2 && k0 < k1) {
+        NS_STAGE(0)
+        if (k0 + kBK < k1) { NS_FETCH(k0 + kBK) }
+    }
+    int buf_at = 0;
     for (int k = k0; k < k1; k += kBK) {
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < N; r++) {
-            const int row = r * 64 + srow, at = spiece ^ ((row >> 2) & 3);
-            u32x4 hi, lo;
-            halves(nl[r][0], nl[r][1], hi, lo);
-            left[0][row][at] = hi;
-            left[1][row][at] = lo;
-            halves(nr[r][0], nr[r][1], hi, lo);
-            const int to = MODE == kApply ? (arow + r * kStride) * kRow + apiece * 16 : row * 64 + at * 16;
-            *reinterpret_cast<u32x4*>(&right[0][to]) = hi;
-            *reinterpret_cast<u32x4*>(&right[1][to]) = lo;
+        if (kD == 1) {
+            NS_STAGE(0)
+            __syncthreads();
+            if (k + kBK < k1) { NS_FETCH(k + kBK) }
         }
-        __syncthreads();
-        if (k + kBK < k1) { NS_FETCH(k + kBK) }
+        const int d = kD == 2 ? buf_at : 0;
 #pragma unroll
         for (int h = 0; h < kBK / 16; h++) {
             f16x8 fl[2][N], fg[2][N];
@@ -320,14 +358,14 @@ __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int
                 const int rl = wi + i * 32 + fr, rr = wj + i * 32 + fr, c = h * 2 + fh;
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    fl[p][i] = __builtin_bit_cast(f16x8, left[p][rl][c ^ ((rl >> 2) & 3)]);
+                    fl[p][i] = __builtin_bit_cast(f16x8, left[d][p][rl][c ^ ((rl >> 2) & 3)]);
                     if (MODE == kApply) {
-                        char* at = &right[p][tr + h * 16 * kRow + i * 64];
+                        char* at = &right[d][p][tr + h * 16 * kRow + i * 64];
                         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
                         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * kRow));
                         fg[p][i] = __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
                     } else {
-                        fg[p][i] = *reinterpret_cast<const f16x8*>(&right[p][rr * 64 + (c ^ ((rr >> 2) & 3)) * 16]);
+                        fg[p][i] = *reinterpret_cast<const f16x8*>(&right[d][p][rr * 64 + (c ^ ((rr >> 2) & 3)) * 16]);
                     }
                 }
             }
@@ -344,6 +382,13 @@ __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int
 #pragma unroll
                     for (int j = 0; j < N; j++)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[o == 0 ? 1 : 0][i], fg[o == 1 ? 1 : 0][j], acc[i][j], 0, 0, 0);
+        }
+        if (kD == 2) {
+            buf_at ^= 1;
+            if (k + kBK < k1) {
+                NS_STAGE(buf_at)
+                if (k + 2 * kBK < k1) { NS_FETCH(k + 2 * kBK) }
+            }
         }
     }
     // a lane holds column j = lane % 32 and rows 8 g + 4 (lane / 32) + 0 .. 3 of each 32 x 32 block
@@ -560,18 +605,24 @@ bool all_small(const pvx_matrix* mats, int count) {
 
 int round_up(int v, int to) { return PVX_CDIV(v, to) * to; }
 
-// 128 x 128 tiles where the largest product has enough of them for the chip, 64 x 64 otherwise
+// 128 x 128 tiles where the widest product fills the chip with them (they read LDS half as often), 64 x 64 otherwise
 int tile_of(const pvx_matrix* mats, int count) {
-    long long tiles = 0;
-    for (int i = 0; i < count; i++) tiles += (long long)PVX_CDIV(mats[i].rows, 128) * PVX_CDIV(mats[i].cols, 128);
-    return tiles >= 256 ? 128 : 64;
+    double tiles = 0.0;
+    for (int i = 0; i < count; i++) tiles += (double)mats[i].rows * mats[i].cols / (128.0 * 128.0);
+    return tiles >= 256.0 ? 128 : 64;
 }
 
-constexpr int kPartWorkgroups = 512;
-
-int parts_of(int want, int k) {          // a part keeps at least four steps
-    const int most = PVX_CDIV(PVX_CDIV(k, kBK), 4);
-    return want < most ? want : most;
+// Parts of a sum: `slots` workgroups run at a time on 256 CUs; the number of parts that leaves the fewest of them idle in the last turn, of
+// those that fit one turn, a part keeping at least four steps of k
+int parts_of(long long tiles, int k, int tile) {
+    const int most = PVX_CDIV(PVX_CDIV(k, kBK), 4), slots = tile == 128 ? 3 : 6;
+    int best = 1;
+    double eff = 0.0;
+    for (int p = 1; p <= most && tiles * p <= 256 * slots; p++) {
+        const double turns = (double)tiles * p / 256.0, e = turns / (double)(long long)(turns + 0.999999);
+        if (e > eff + 0.02) { eff = e; best = p; }
+    }
+    return best;
 }
 
 void fill(Table& t, const pvx_matrix* mats, int count, int tile, size_t* total) {
@@ -589,12 +640,10 @@ void fill(Table& t, const pvx_matrix* mats, int count, int tile, size_t* total) 
         q.np = round_up(q.n, tile);
         tiles += (long long)(q.mp / tile) * (q.mp / tile + 1) / 2;
     }
-    // a sum is cut in parts where the batch has fewer tiles than fill the chip
-    const int want = (int)PVX_CDIV((long long)kPartWorkgroups, tiles < 1 ? 1 : tiles);
     for (int i = 0; i < count; i++) {
         Mat& q = t.mat[i];
-        q.parts = parts_of(want, q.n);
-        q.parts2 = parts_of(want, q.m);
+        q.parts = parts_of(tiles, q.n, tile);
+        q.parts2 = parts_of(tiles, q.m, tile);
         q.base = (long long)off;
         const size_t px = (size_t)q.mp * q.np, pa = (size_t)q.mp * q.mp, lower = (size_t)(q.mp / tile) * (q.mp / tile + 1) / 2 * tile * tile;
         const int parts = q.parts > q.parts2 ? q.parts : q.parts2;
@@ -629,7 +678,7 @@ int run(Table& t, char* ws, int steps, float a, float b, float c, float eps, hip
                   const long long k = PVX_CDIV((long long)q.m * q.n, (long long)kNormChunk);
                   return k > kNormBlocks ? (long long)kNormBlocks : k;
               }), T);
-    NS_LAUNCH((ns_load_kernel<E>), ([](const Mat& q) { return (long long)(q.mp / 64) * (q.np / 64); }), T, eps, steps, a, b, c);
+    NS_LAUNCH((ns_load_kernel<E>), ([](const Mat& q) { return (long long)(q.mp / 64) * (q.np / 64); }), T, eps, steps, poly_of(a, b, c));
     if (steps == 0) NS_LAUNCH((ns_store_kernel<E>), ([](const Mat& q) { return PVX_CDIV((long long)q.m * q.n, (long long)kBlk); }), T);
     for (int s = 0; s < steps; s++) {
         const int last = s == steps - 1;

@@ -107,21 +107,17 @@ def sort_index(index, num_rows):
     num_rows = int(num_rows)
     if num_rows < 1:
         raise ValueError("num_rows must be at least 1, got %d" % num_rows)
-    return _sort(index.reshape(-1).contiguous(), num_rows)
-
-
-def _sort(index, num_rows, want_offsets=True):
-    """index [n] contiguous"""
+    index = index.reshape(-1).contiguous()
     n, dev = index.shape[0], index.device
     L = _lib.lib()
     with _lib.on(dev):
         order = torch.empty(n, dtype=torch.int32, device=dev)
         keys = torch.empty(n, dtype=torch.int32, device=dev)
-        offsets = torch.empty(num_rows + 1, dtype=torch.int32, device=dev) if want_offsets else None
+        offsets = torch.empty(num_rows + 1, dtype=torch.int32, device=dev)
         size = L.pvx_sort_index_workspace_bytes(n)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         rc = L.pvx_sort_index(index.data_ptr(), index.dtype == torch.int64, n, num_rows, order.data_ptr(), keys.data_ptr(),
-                              offsets.data_ptr() if want_offsets else None, ws.data_ptr(), size, _lib.raw_stream(dev))
+                              offsets.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
         if rc:
             _lib.check(rc, "pvx_sort_index")
     return IndexSort(order, keys, offsets, num_rows)
@@ -158,10 +154,11 @@ class _LookupRows(torch.autograd.Function):
         if m > 0 and w > 0:
             L = _lib.lib()
             with _lib.on(dev):
-                sort = ctx.sort if ctx.sort is not None else _sort(index, m, want_offsets=False)
-                size = L.pvx_lookup_rows_grad_workspace_bytes(n, w)
+                sort = ctx.sort
+                size = L.pvx_lookup_rows_grad_workspace_bytes(n, w, sort is not None)
                 ws = torch.empty(size, dtype=torch.uint8, device=dev)
-                rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], sort.order.data_ptr(), sort.keys.data_ptr(),
+                order, keys = (sort.order.data_ptr(), sort.keys.data_ptr()) if sort is not None else (None, None)
+                rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], index.data_ptr(), index.dtype == torch.int64, order, keys,
                                             n, m, w, ctx.scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
                 if rc:
                     _lib.check(rc, "pvx_lookup_rows_grad")

@@ -1,7 +1,8 @@
 """Newton-Schulz orthogonalisation (csrc/orthogonalize.hip; optim.orthogonalize, optim.Muon) against the iteration in float64.
 
 Tolerance.  A step is X <- p(X X^T) X with |p| <= a + |b| + |c| on [0, 1.3].  Let d be the relative error of a product's operands
-(2^-24 for three planes, 2^-17 for two): it enters X at most three times a step (A, A A, B X), scaled by at most a + 2 |b| + 3 |c| = 19 of
+(two f16 halves hold 22 bits and the sign of the second one: at most 2^-22, 2^-24 in the root mean square, the dropped product of the
+second halves included, whatever the matrices' dtype): it enters X at most three times a step (A, A A, B X), scaled by at most a + 2 |b| + 3 |c| = 19 of
 the value it enters, and the later steps carry it with a gain of at most a = 3.4445 each (the polynomial's slope at 0 is its largest on
 the range).  Over five steps that is at most 19 (1 + .. + 3.4445^4) d = 19 * 198 d <= 3800 d relative to the result: `bound(.., tight=False)`,
 for any spectrum.  Where no direction is amplified by more than the result itself (random matrices at least twice as wide as high: all
@@ -38,7 +39,7 @@ def rel(got, want):
 
 
 def bound(dtype, tight, shape=(1, 1)):
-    d, m, n = (2.0 ** -24 if dtype == torch.float32 else 2.0 ** -17), min(shape), max(shape)
+    d, m, n = 2.0 ** -24, min(shape), max(shape)
     sums = 5 * ((6 * n / 16) ** 0.5 + 2 * (6 * m / 16) ** 0.5) * 2.0 ** -24
     return (40 if tight else 3800) * d + sums + torch.finfo(dtype).eps / 2
 

@@ -57,12 +57,15 @@ def test_lookup_codes():
     assert sort(n=0x7fffffff) == RANGE and sort(m=0x7fffffff) == RANGE
     assert sort(n=100000, m=50) == WORKSPACE and sort(n=100000, ws=None, size=1 << 30) == WORKSPACE
     assert L.pvx_sort_index_workspace_bytes(100000) > 3 * 4 * 100000 and L.pvx_sort_index_workspace_bytes(0) == 256
-    grad = lambda dout=P, dtype=0, order=P, keys=P, n=5000, m=4, w=8, out=P, ws=P, size=0: L.pvx_lookup_rows_grad(  # noqa: E731
-        dout, dtype, order, keys, n, m, w, 1.0, out, ws, size, None)
-    for kw in (dict(n=-1), dict(m=-1), dict(w=-1), dict(dtype=9), dict(dout=None), dict(order=None), dict(keys=None), dict(out=None)):
+    grad = lambda dout=P, dtype=0, index=P, order=P, keys=P, n=5000, m=4, w=8, out=P, ws=P, size=0: L.pvx_lookup_rows_grad(  # noqa: E731
+        dout, dtype, index, 0, order, keys, n, m, w, 1.0, out, ws, size, None)
+    for kw in (dict(n=-1), dict(m=-1), dict(w=-1), dict(dtype=9), dict(dout=None), dict(order=None), dict(keys=None), dict(out=None),
+               dict(index=None, order=None, keys=None)):
         assert grad(**kw) == INVALID, kw
-    assert grad(m=0) == 0 and grad(w=0) == 0 and grad() == WORKSPACE and grad(n=0x7fffffff) == RANGE
-    assert L.pvx_lookup_rows_grad_workspace_bytes(5000, 8) > 5000 // 64 * 8 * 4
+    assert grad(m=0) == 0 and grad(w=0) == 0 and grad() == WORKSPACE and grad(order=None, keys=None) == WORKSPACE and grad(n=0x7fffffff) == RANGE
+    sorted_bytes = L.pvx_lookup_rows_grad_workspace_bytes(5000, 8, 1)
+    assert sorted_bytes > 5000 // 64 * 8 * 4 and L.pvx_lookup_rows_grad_workspace_bytes(5000, 8, 0) > sorted_bytes + 2 * 4 * 5000
+    assert grad(order=None, keys=None, size=sorted_bytes) == WORKSPACE
 
 
 def test_python_refuses_cpu_tensors():
