@@ -214,8 +214,8 @@ _HERE_ALREADY = _Here()
 
 
 def on(device):
-    """`with on(tensor.device) as ..`: torch.cuda.device, without its cost where the device is the current one already"""
-    return _HERE_ALREADY if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    """`with on(tensor.device):` is torch.cuda.device, without its cost where the device is the current one already"""
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def raw_stream(device):

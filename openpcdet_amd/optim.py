@@ -20,14 +20,17 @@ def _launch(mats, outs, steps, coefficients, eps):
     L = _lib.lib()
     dev, code = mats[0].device, _lib.DTYPE_CODE[mats[0].dtype]
     a, b, c = coefficients
-    with torch.cuda.device(dev):
-        stream = _lib.stream()
+    with _lib.on(dev):
+        stream = _lib.raw_stream(dev)
         for at in range(0, len(mats), MAX_MATRICES):
             part = [v for m, o in zip(mats[at:at + MAX_MATRICES], outs[at:at + MAX_MATRICES]) for v in (m.data_ptr(), o.data_ptr(), *m.shape)]
             count = len(part) // 4
             table = struct.pack("QQii" * count, *part)
-            ws = _lib.workspace(L.pvx_orthogonalize_workspace_bytes(table, count, code), dev)
-            _lib.check(L.pvx_orthogonalize(table, count, code, steps, a, b, c, eps, _lib.ptr(ws), ws.numel(), stream), "pvx_orthogonalize")
+            size = L.pvx_orthogonalize_workspace_bytes(table, count, code)
+            ws = mats[0].new_empty(size, dtype=torch.uint8)
+            rc = L.pvx_orthogonalize(table, count, code, steps, a, b, c, eps, ws.data_ptr(), size, stream)
+            if rc:
+                _lib.check(rc, "pvx_orthogonalize")
 
 
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -58,7 +61,7 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
             whole = torch.empty(matrices.shape, dtype=matrices.dtype, device=matrices.device)
             outs = list(whole.unbind(0))
         else:
-            outs = [torch.empty(m.shape, dtype=m.dtype, device=m.device) for m in mats]
+            outs = [m.new_empty(m.shape) for m in mats]
         for m, o in zip(mats, outs):
             if m.numel() > 0:
                 g = groups.setdefault((m.dtype, m.device), ([], []))

@@ -128,7 +128,7 @@ def _lookup(table, index, scale):
     n, (m, w) = index.shape[0], table.shape
     dev = table.device
     with _lib.on(dev):
-        out = torch.empty((n, w), dtype=table.dtype, device=dev)
+        out = table.new_empty((n, w))
         rc = _lib.lib().pvx_lookup_rows(table.data_ptr(), _lib.DTYPE_CODE[table.dtype], index.data_ptr(), index.dtype == torch.int64, n, m, w, scale,
                                         out.data_ptr(), _lib.raw_stream(dev))
         if rc:
@@ -144,25 +144,30 @@ class _LookupRows(torch.autograd.Function):
         return _lookup(table, index, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        index, = ctx.saved_tensors
-        m, w = ctx.shape
-        n, dev = index.shape[0], index.device
-        grad = grad.contiguous()
-        dtable = torch.empty((m, w), dtype=grad.dtype, device=dev)
-        if m > 0 and w > 0:
-            L = _lib.lib()
-            with _lib.on(dev):
-                sort = ctx.sort
-                size = L.pvx_lookup_rows_grad_workspace_bytes(n, w, sort is not None)
-                ws = torch.empty(size, dtype=torch.uint8, device=dev)
-                order, keys = (sort.order.data_ptr(), sort.keys.data_ptr()) if sort is not None else (None, None)
-                rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], index.data_ptr(), index.dtype == torch.int64, order, keys,
-                                            n, m, w, ctx.scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
-                if rc:
-                    _lib.check(rc, "pvx_lookup_rows_grad")
-        return dtable, None, None, None
+        return _lookup_grad_once(ctx, grad) if torch.is_grad_enabled() else _lookup_grad(ctx, grad)
+
+
+def _lookup_grad(ctx, grad):
+    index, = ctx.saved_tensors
+    m, w = ctx.shape
+    n, dev, sort = index.shape[0], index.device, ctx.sort
+    grad = grad.contiguous()
+    dtable = grad.new_empty((m, w))
+    if m > 0 and w > 0:
+        L = _lib.lib()
+        with _lib.on(dev):
+            size = L.pvx_lookup_rows_grad_workspace_bytes(n, w, sort is not None)
+            ws = grad.new_empty(size, dtype=torch.uint8)
+            order, keys = (sort.order.data_ptr(), sort.keys.data_ptr()) if sort is not None else (None, None)
+            rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], index.data_ptr(), index.dtype == torch.int64, order, keys,
+                                        n, m, w, ctx.scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
+            if rc:
+                _lib.check(rc, "pvx_lookup_rows_grad")
+    return dtable, None, None, None
+
+
+_lookup_grad_once = once_differentiable(_lookup_grad)      # under create_graph: a second derivative is refused, not left out
 
 
 def lookup_rows(table, index, scale=1.0, sort=None):

@@ -196,9 +196,9 @@ def _group_norm_fwd(x, weight, bias, residual, offsets, order, samples, groups, 
     dev = x.device
     with _lib.on(dev):
         y = torch.empty_like(x)
-        stats = torch.empty((2, samples, groups), dtype=torch.float32, device=dev)
+        stats = x.new_empty((2, samples, groups), dtype=torch.float32)
         size = L.pvx_group_norm_act_workspace_bytes(n, c, samples, offsets is not None, groups)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        ws = x.new_empty(size, dtype=torch.uint8)
         base = stats.data_ptr()
         rc = L.pvx_group_norm_act_fwd(x.data_ptr(), n, c, _lib.DTYPE_CODE[x.dtype], samples, _addr(offsets), _addr(order), groups, _addr(weight),
                                       _addr(bias), _param_code(weight, bias), eps, _addr(residual), act, y.data_ptr(), base,
@@ -222,29 +222,35 @@ class _GroupNormAct(Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, residual, offsets, order, stats = ctx.saved_tensors
-        samples, groups, act = ctx.args
-        L = _lib.lib()
-        n, c = x.shape
-        dev = x.device
-        dy = dy.contiguous()
-        with _lib.on(dev):
-            dx = torch.empty_like(x)
-            dres = torch.empty_like(x) if residual is not None else None
-            dw = torch.empty_like(weight) if weight is not None else None
-            db = torch.empty_like(bias) if bias is not None else None
-            size = L.pvx_group_norm_act_workspace_bytes(n, c, samples, offsets is not None, groups)
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            base = stats.data_ptr()
-            rc = L.pvx_group_norm_act_bwd(dy.data_ptr(), x.data_ptr(), _addr(residual), n, c, _lib.DTYPE_CODE[x.dtype], samples, _addr(offsets),
-                                          _addr(order), groups, _addr(weight), _addr(bias), _param_code(weight, bias), base,
-                                          base + 4 * samples * groups, act, dx.data_ptr(), _addr(dres), _addr(dw), _addr(db), ws.data_ptr(), size,
-                                          _lib.raw_stream(dev))
-            if rc:
-                _lib.check(rc, "pvx_group_norm_act_bwd")
-        return dx, dw, db, dres, None, None, None, None, None, None
+        return _group_norm_bwd_once(ctx, dy) if torch.is_grad_enabled() else _group_norm_bwd(ctx, dy)
+
+
+def _group_norm_bwd(ctx, dy):
+    x, weight, bias, residual, offsets, order, stats = ctx.saved_tensors
+    samples, groups, act = ctx.args
+    L = _lib.lib()
+    n, c = x.shape
+    dev = x.device
+    dy = dy.contiguous()
+    with _lib.on(dev):
+        dx = torch.empty_like(x)
+        dres = torch.empty_like(x) if residual is not None else None
+        dw = torch.empty_like(weight) if weight is not None else None
+        db = torch.empty_like(bias) if bias is not None else None
+        size = L.pvx_group_norm_act_workspace_bytes(n, c, samples, offsets is not None, groups)
+        ws = x.new_empty(size, dtype=torch.uint8)
+        base = stats.data_ptr()
+        rc = L.pvx_group_norm_act_bwd(dy.data_ptr(), x.data_ptr(), _addr(residual), n, c, _lib.DTYPE_CODE[x.dtype], samples, _addr(offsets),
+                                      _addr(order), groups, _addr(weight), _addr(bias), _param_code(weight, bias), base,
+                                      base + 4 * samples * groups, act, dx.data_ptr(), _addr(dres), _addr(dw), _addr(db), ws.data_ptr(), size,
+                                      _lib.raw_stream(dev))
+        if rc:
+            _lib.check(rc, "pvx_group_norm_act_bwd")
+    return dx, dw, db, dres, None, None, None, None, None, None
+
+
+_group_norm_bwd_once = once_differentiable(_group_norm_bwd)      # under create_graph: a second derivative is refused, not left out
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, residual=None, offsets=None, order=None):
