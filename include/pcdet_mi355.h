@@ -582,10 +582,14 @@ int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, 
  *   X = M / (|M|_F + eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X;   out = X in the matrix's own orientation
  * mats: HOST array; in and out are device pointers to contiguous row-major matrices (they may be the same).  The
  * products have the accuracy of binary32, whatever the dtype.  rows, cols <= 2^20, steps <= 64.
+ * The products keep their operands against a bound of the singular values that is followed through the steps.  Coefficients for which
+ * that bound says too little (from a start in [1/64, 1] it leaves a factor of 128 between the largest value's bounds, or passes 10^9)
+ * are PVX_ERR_RANGE; pvx_orthogonalize_holds is 1 for those that are taken.
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct { const void* in; void* out; int rows, cols; } pvx_matrix;
 #define PVX_ORTHO_MAX 64
 size_t pvx_orthogonalize_workspace_bytes(const pvx_matrix* mats, int count, int dtype);
+int pvx_orthogonalize_holds(int steps, float a, float b, float c);
 int pvx_orthogonalize(const pvx_matrix* mats, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace,
                       size_t workspace_bytes, void* stream);
 

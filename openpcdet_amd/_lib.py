@@ -64,6 +64,7 @@ SIGNATURES = {
                                        c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                        c_size_t, c_void_p]),
     "pvx_orthogonalize_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int]),
+    "pvx_orthogonalize_holds": (c_int, [c_int, c_float, c_float, c_float]),
     "pvx_orthogonalize": (c_int, [c_void_p, c_int, c_int, c_int, c_float, c_float, c_float, c_float, c_void_p, c_size_t, c_void_p]),
     "pvx_points_transform": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "pvx_boxes_transform": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),

@@ -161,6 +161,37 @@ Poly poly_of(float a, float b, float c) {
     return p;
 }
 
+// Whether the followed bound says enough about the values.  The largest singular value starts between 1 / 64 (4096 equal ones) and 1
+// times the norm; [lo, r] is what a step makes of that range, r with the 1 % that the scales take.  f16 has 2^-39 of its bound as half
+// its last step, so with r <= 128 lo an entry of A, kept against r^2, is off by at most 2^-25 of the square of the largest value: as
+// binary32.  3 x - 2 x^3 shows what must not pass: the values stay below sqrt(2), at whose end the slope is -9, but 1 % more makes the
+// bound 1.4, 1.6, 2.9, 39, 1e5, and everything is lost below f16's last step.  A norm near eps starts lower: 2^0, 2^-2, .. 2^-20.
+bool bound_holds(int steps, float a, float b, float c) {
+    constexpr double kSpread = 128.0, kMost = 1e9;       // kMost: where above() ends
+    const Poly p = poly_of(a, b, c);
+    auto f = [&](double x) { return x * (a + x * x * (b + x * x * (double)c)); };
+    for (int e = 0; e <= 20; e += 2) {
+        double lo = ldexp(1.0 / 64.0, -e), r = ldexp(1.01, -e);
+        for (int s = 0; s < steps; s++) {
+            double at[4] = {lo, lo, lo, r};              // f is monotonic between these
+            for (int i = 0; i < 2; i++)
+                if (p.x[i] > lo && p.x[i] < r) at[1 + i] = p.x[i];
+            if (at[1] > at[2]) { const double x = at[1]; at[1] = at[2]; at[2] = x; }
+            double least = fabs(f(lo)), most = least;
+            for (int i = 1; i < 4; i++) {
+                const double v = f(at[i]);
+                if (v * f(at[i - 1]) < 0.0) least = 0.0;
+                least = fmin(least, fabs(v));
+                most = fmax(most, fabs(v));
+            }
+            lo = least;
+            r = 1.01 * most;
+            if (r > kSpread * lo || r > kMost) return false;
+        }
+    }
+    return true;
+}
+
 // the power of two above `most`, within what the scales can hold; 0 and NaN: anything will do
 __device__ __forceinline__ int above(float most) {
     if (!(most > 1e-30f)) return most > 0.f ? -99 : 0;
@@ -657,7 +688,7 @@ template <typename F> int spread(Table& t, F blocks) {
     for (int i = 0; i < t.count; i++) {
         t.first[i] = (int)at;
         at += blocks(t.mat[i]);
-        if (at > 0x7fffffffLL) return -1;
+        if (at > 0xffffffLL) return -1;                  // workgroups x threads stay below 2^32
     }
     t.first[t.count] = (int)at;
     return (int)at;
@@ -711,12 +742,16 @@ extern "C" size_t pvx_orthogonalize_workspace_bytes(const pvx_matrix* mats, int 
     return total;
 }
 
+extern "C" int pvx_orthogonalize_holds(int steps, float a, float b, float c) {
+    return steps >= 0 && steps <= kMaxSteps && bound_holds(steps, a, b, c);
+}
+
 extern "C" int pvx_orthogonalize(const pvx_matrix* mats, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace,
                                  size_t workspace_bytes, void* stream) {
     const int bad = check_args(mats, count, dtype);
     if (bad != PVX_OK) return bad;
     if (steps < 0 || !(eps >= 0.f)) return PVX_ERR_INVALID;
-    if (steps > kMaxSteps) return PVX_ERR_RANGE;
+    if (steps > kMaxSteps || !bound_holds(steps, a, b, c)) return PVX_ERR_RANGE;
     if (count == 0) return PVX_OK;
     for (int i = 0; i < count; i++)
         if (!mats[i].in || !mats[i].out) return PVX_ERR_INVALID;

@@ -30,7 +30,13 @@ def _launch(mats, outs, steps, coefficients, eps):
             ws = mats[0].new_empty(size, dtype=torch.uint8)
             rc = L.pvx_orthogonalize(table, count, code, steps, a, b, c, eps, ws.data_ptr(), size, stream)
             if rc:
+                _check_coefficients(steps, coefficients)
                 _lib.check(rc, "pvx_orthogonalize")
+
+
+def _check_coefficients(steps, coefficients):
+    if not _lib.lib().pvx_orthogonalize_holds(steps, *coefficients):
+        raise ValueError("%d steps of the coefficients %r do not keep the singular values within known bounds" % (steps, tuple(coefficients)))
 
 
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -38,7 +44,9 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     X = M / (|M|_F + eps) (with the shorter side first), (a, b, c) = coefficients: the singular vectors of M with singular values near 1.
 
     matrices: a matrix [r, c], a batch of them [B, r, c], or a list or tuple of matrices of any sizes; float32 / float16 / bfloat16, on the
-    GPU.  The result has the same form, in the inputs' dtypes; whatever they are, the products are as accurate as binary32's.  No gradient flows through it.  Matrices of one dtype go through the GPU together, up to 64 in a call."""
+    GPU.  The result has the same form, in the inputs' dtypes; whatever they are, the products are as accurate as binary32's.  No gradient flows through it.
+    Matrices of one dtype go through the GPU together, up to 64 in a call.  Coefficients whose polynomial does not keep the singular values
+    within known bounds over the steps (a root or a fixed point that repels inside [0, 1], or growth past 1e9) are refused."""
     one = isinstance(matrices, torch.Tensor)
     if one and matrices.dim() not in (2, 3):
         raise ValueError("a matrix [r, c] or a batch [B, r, c] is wanted, got %s" % (tuple(matrices.shape),))
@@ -84,6 +92,7 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("lr and weight_decay must not be negative and momentum must be in [0, 1): got %r, %r, %r" % (lr, weight_decay, momentum))
         if not 0 <= int(steps) <= MAX_STEPS or not eps >= 0.0 or len(coefficients) != 3:
             raise ValueError("steps must be 0 .. %d and eps not negative, with three coefficients: got %r, %r, %r" % (MAX_STEPS, steps, eps, coefficients))
+        _check_coefficients(int(steps), coefficients)
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps),
                                       coefficients=tuple(coefficients), eps=eps))
 

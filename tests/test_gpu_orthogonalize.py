@@ -93,6 +93,15 @@ def test_steps_and_scale(cuda_device):
     m[3, 4] = float("nan")
     both = optim.orthogonalize([m, m[:, 10:]])
     assert bool(torch.isnan(both[0]).all()) and bool(torch.isfinite(both[1]).all())
+    big = torch.randn(70, 300, device=cuda_device)
+    big[3, 4] = float("inf")
+    assert bool(torch.isnan(optim.orthogonalize(big)).all())
+    for grow in ((4.0, 0.0, 0.0), (0.5, 0.0, 0.0)):                      # coefficients that let the values grow or fall: the scales follow
+        assert rel(optim.orthogonalize(big[10:], steps=6, coefficients=grow), reference(big[10:], 6, coefficients=grow)) <= 100 * 2.0 ** -24
+    # 3 x - 2 x^3 keeps [0, sqrt(2)], but its slope at that end is 3 - 6 * 2 = -9: with 1 % to spare a step the bound of the values goes
+    # 1.43, 1.56, 2.9, 39, 1.2e5, 3.7e15 while they stay below 1.42, and words kept against it hold nothing.  Refused, not computed wrongly.
+    with pytest.raises(ValueError, match="bounds"):
+        optim.orthogonalize(big[10:], steps=6, coefficients=(3.0, -2.0, 0.0))
 
 
 def test_lists_batches_and_strides(cuda_device):

@@ -88,6 +88,19 @@ def test_modules_refuse():
     assert norm.act_name(torch.nn.GELU("tanh")) is None and norm.act_name(torch.nn.GELU()) == "gelu" and norm.act_name(torch.nn.ReLU6()) is None
 
 
+@pytest.mark.parametrize("co, steps, holds", [
+    (optim.COEFFICIENTS, 5, 1), (optim.COEFFICIENTS, 64, 1), ((1.5, -0.5, 0.0), 64, 1), ((1.875, -1.25, 0.375), 64, 1), ((2.0, -1.5, 0.5), 64, 1),
+    ((4.0, 0.0, 0.0), 6, 1), ((4.0, 0.0, 0.0), 16, 0), ((0.5, 0.0, 0.0), 64, 1), ((0.0, 0.0, 0.0), 3, 1), ((3.0, -2.0, 0.0), 0, 1),
+    ((3.0, -2.0, 0.0), 6, 0), ((0.5, 1.0, 0.0), 4, 0), ((1.0, -1.0, 0.0), 1, 0), (optim.COEFFICIENTS, 65, 0), (optim.COEFFICIENTS, -1, 0)])
+def test_orthogonalize_coefficients(co, steps, holds):
+    """4^16 > 1e9; 3 x - 2 x^3 and x - x^3 have a root in (0, 1.01 ..]; x / 2 + x^3 leaves 0.7 to either side."""
+    assert _lib.lib().pvx_orthogonalize_holds(steps, *co) == holds
+    if not holds and 0 <= steps <= optim.MAX_STEPS:
+        assert _lib.lib().pvx_orthogonalize(None, 0, 0, steps, *co, 1e-7, None, 0, None) == RANGE
+        with pytest.raises(ValueError, match="bounds"):
+            optim.Muon([torch.nn.Parameter(torch.zeros(4, 4))], steps=steps, coefficients=co)
+
+
 def test_orthogonalize_codes():
     L = _lib.lib()
     call = lambda mats, count=None, dtype=0, steps=5, eps=1e-7, ws=P, size=0: L.pvx_orthogonalize(  # noqa: E731
