@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kBlk) void run_sum_kernel(const E* __restrict__ dou
                     for (int j = 0; j < V; j++) acc[j] += (float)q[u].e[j];
                     const bool last = at == p1 - 1;
                     if (!last && key[u + 1] == v) continue;
-                    if (v < m) {
+                    if ((unsigned)v < (unsigned)m) {
                         const bool from_left = begin == p0 && left == v, to_right = last && right == v;
                         if (!from_left && !to_right) {
                             store_row<E, V>(dtable, (long long)v * ch + k, acc, scale);
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(kBlk) void run_next_kernel(const float* __restrict_
         for (long long blk = t.first(); blk < blocks; blk += t.step()) {
             const long long p0 = blk << shift;
             const int key = keys[p0];
-            if (key >= m || keys[p0 + (1LL << shift) - 1] != key) continue;
+            if ((unsigned)key >= (unsigned)m || keys[p0 + (1LL << shift) - 1] != key) continue;
             float acc = 0.f;
 #pragma unroll 16
             for (int i = 0; i < kFan; i++) acc += in[(blk * kFan + i) * width + k];
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ 
     for (int k = t.chunk; k < ch; k += kBlk) {
         for (long long blk = t.first(); blk < blocks - 1; blk += t.step()) {
             const int p0 = (int)blk * kFan, v = keys[p0 + kFan - 1];
-            if (v >= m || keys[p0 + kFan] != v) continue;
+            if ((unsigned)v >= (unsigned)m || keys[p0 + kFan] != v) continue;
             const bool whole = keys[p0] == v;
             if (whole && p0 > 0 && keys[p0 - 1] == v) continue;                  // it began further left
             const float* q = (whole ? lv.p[0] : lv.tail) + (blk * ch + k) * V;
