@@ -267,27 +267,27 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 __global__ __launch_bounds__(kBlk) void gn_finish_kernel(const double* __restrict__ partial, Rows rows, int c, int groups, int units, int range,
                                                           float eps, float* __restrict__ mean, float* __restrict__ rstd) {
     __shared__ double red[kWaves];
-    const int s = blockIdx.x / groups, g = blockIdx.x % groups, cpg = c / groups;
-    const int lo = rows.begin(s), hi = rows.begin(s + 1);
-    double a = 0.0, b = 0.0;
-    if (hi > lo) {
-        const int k0 = lo / range, pieces = (hi - 1) / range - k0 + 1;
-        const int upg = units / groups;
-        for (int i = threadIdx.x; i < pieces * upg; i += kBlk) {
-            const double* q = partial + ((size_t)(k0 + s + i / upg) * units + g * upg + i % upg) * 2;
-            a += q[0];
-            b += q[1];
+    const int cpg = c / groups, upg = units / groups;
+    for (int pair = blockIdx.x; pair < rows.samples * groups; pair += gridDim.x) {
+        const int s = pair / groups, g = pair % groups, lo = rows.begin(s), hi = rows.begin(s + 1);
+        double a = 0.0, b = 0.0;
+        if (hi > lo) {
+            const int k0 = lo / range, pieces = (hi - 1) / range - k0 + 1;
+            for (int i = threadIdx.x; i < pieces * upg; i += kBlk) {
+                const double2 q = *reinterpret_cast<const double2*>(partial + ((size_t)(k0 + s + i / upg) * units + g * upg + i % upg) * 2);
+                a += q.x;
+                b += q.y;
+            }
         }
+        a = block_sum(a, red);
+        b = block_sum(b, red);
+        if (threadIdx.x != 0) continue;
+        const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0, mu = a / count;
+        double var = b / count - mu * mu;
+        if (var < 0.0) var = 0.0;
+        mean[pair] = (float)mu;
+        rstd[pair] = (float)(1.0 / sqrt(var + (double)eps));
     }
-    a = block_sum(a, red);
-    b = block_sum(b, red);
-    if (threadIdx.x != 0) return;
-    const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
-    const double mu = a / count;
-    double var = b / count - mu * mu;
-    if (var < 0.0) var = 0.0;
-    mean[blockIdx.x] = (float)mu;
-    rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)eps));
 }
 
 // a thread's channels of one sample
@@ -498,17 +498,19 @@ __device__ __forceinline__ void channel_finish(const double* partial, const Rows
     }
 }
 
-// backward, finish: workgroups 0 .. samples * groups - 1 leave mean gx and mean(gx xhat) of their (sample, group); the c behind them
-// leave db and dw of their channel, summed over the pieces in order
+// backward, finish: mean gx and mean(gx xhat) of each (sample, group), and behind them db and dw of each channel
 __global__ __launch_bounds__(kBlk) void gn_bwd_finish_kernel(const double* __restrict__ partial, Rows rows, int c, int groups, int range,
                                                               const void* __restrict__ weight, int pd, float* __restrict__ m0,
                                                               float* __restrict__ m1, void* __restrict__ dweight, void* __restrict__ dbias) {
     __shared__ double red[kWaves];
     const int pairs = rows.samples * groups, cpg = c / groups;
-    double a = 0.0, b = 0.0;
-    if ((int)blockIdx.x < pairs) {
-        const int s = blockIdx.x / groups, g = blockIdx.x % groups;
-        const int lo = rows.begin(s), hi = rows.begin(s + 1);
+    for (int pair = blockIdx.x; pair < pairs + c; pair += gridDim.x) {
+        if (pair >= pairs) {
+            channel_finish(partial, rows, c, range, pair - pairs, pd, dweight, dbias, red);
+            continue;
+        }
+        const int s = pair / groups, g = pair % groups, lo = rows.begin(s), hi = rows.begin(s + 1);
+        double a = 0.0, b = 0.0;
         if (hi > lo) {
             const int k0 = lo / range, pieces = (hi - 1) / range - k0 + 1;
             for (int i = threadIdx.x; i < pieces * cpg; i += kBlk) {
@@ -523,12 +525,10 @@ __global__ __launch_bounds__(kBlk) void gn_bwd_finish_kernel(const double* __res
         b = block_sum(b, red);
         if (threadIdx.x == 0) {
             const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
-            m0[blockIdx.x] = (float)(a / count);
-            m1[blockIdx.x] = (float)(b / count);
+            m0[pair] = (float)(a / count);
+            m1[pair] = (float)(b / count);
         }
-        return;
     }
-    channel_finish(partial, rows, c, range, blockIdx.x - pairs, pd, dweight, dbias, red);
 }
 
 // dx (and dresidual) of a workgroup's positions.  With `gpart` the two means are finished here, and the workgroups behind the `blocks`
@@ -885,6 +885,8 @@ int check_args(int n, int c, int dtype, int samples, const int* offsets, int gro
     return PVX_OK;
 }
 
+dim3 finish_grid(long long results) { return dim3((unsigned)(results < 65536 ? results : 65536)); }
+
 #define GN_DISPATCH(E, v, CALL)                                                            \
     do {                                                                                   \
         if (v == 4) { CALL(E, 4); }                                                        \
@@ -922,7 +924,7 @@ int fwd_impl(const void* x, const Rows& rows, int c, int groups, const void* wei
     GN_DISPATCH(E, sh.v, GN_SUMS);
     PVX_CHECK_LAUNCH();
     if (!sh.merged) {
-        hipLaunchKernelGGL(gn_finish_kernel, dim3(rows.samples * groups), dim3(kBlk), 0, st, ws.partial, rows, c, groups, units, sh.range, eps, mean, rstd);
+        hipLaunchKernelGGL(gn_finish_kernel, finish_grid((long long)rows.samples * groups), dim3(kBlk), 0, st, ws.partial, rows, c, groups, units, sh.range, eps, mean, rstd);
         PVX_CHECK_LAUNCH();
     }
 #define GN_APPLY_ACT(E, V, A) hipLaunchKernelGGL((gn_apply_kernel<E, V, A>), grid, dim3(kBlk), sh.merged ? lds : 0, st, (const E*)x,         \
@@ -966,7 +968,7 @@ int bwd_impl(const void* dy, const void* x, const void* residual, const Rows& ro
     GN_DISPATCH(E, sh.v, GN_BSUMS);
     PVX_CHECK_LAUNCH();
     if (!sh.merged) {
-        hipLaunchKernelGGL(gn_bwd_finish_kernel, dim3(rows.samples * groups + c), dim3(kBlk), 0, st, ws.partial, rows, c, groups, sh.range, weight, pd,
+        hipLaunchKernelGGL(gn_bwd_finish_kernel, finish_grid((long long)rows.samples * groups + c), dim3(kBlk), 0, st, ws.partial, rows, c, groups, sh.range, weight, pd,
                            ws.m0, ws.m1, dweight, dbias);
         PVX_CHECK_LAUNCH();
     }

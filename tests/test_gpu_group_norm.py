@@ -155,6 +155,13 @@ def test_odd_shapes(cuda_device, n, c, groups, cuts):
         check(cuda_device, n, c, groups, cuts=cuts, dtype=dtype, act="silu", eps=1e-3)
 
 
+def test_many_groups_and_samples(cuda_device):
+    check(cuda_device, 20000, 2048, 2048, cuts=[0, 20000], act="silu")                   # a group a channel: the widest workgroup's LDS
+    check(cuda_device, 20000, 2048, 1, cuts=[0, 9000, 20000], act="silu")
+    check(cuda_device, 3000, 1024, 1024, cuts=[0, 3000], dtype=torch.bfloat16)
+    check(cuda_device, 60000, 4, 4, cuts=[0] + sorted(torch.randint(0, 60000, (2999,), generator=torch.Generator().manual_seed(1)).tolist()) + [60000], eps=1e-2)      # 3000 frames
+
+
 def test_rows_of_no_sample(cuda_device):
     check(cuda_device, 120, 16, 2, cuts=[10, 50, 100], act="gelu", res=True)              # one launch
     check(cuda_device, 9000, 16, 2, cuts=[100, 5000, 8000], act="gelu", res=True)
@@ -308,6 +315,8 @@ def test_sparse_module_and_sequential(cuda_device):
         out.features.square().sum().backward()
         assert float(f.grad.abs().sum()) > 0 and gn.weight.grad is not None
         assert torch.equal(seq.eval()(x).features, out.features)          # nothing depends on the mode
+    none = spconv.SparseConvTensor(feats[:0].requires_grad_(True), idx[:0], [8, 20, 20], 3)
+    assert spconv.SparseSequential(spconv.SparseGroupNorm(4, 16).to(cuda_device), torch.nn.ReLU())(none).features.shape == (0, 16)
     assert x._sample_rows()[0].tolist()[1] == x._sample_rows()[0].tolist()[2]
     first = x._sample_rows()
     assert x._sample_rows()[0] is first[0] and x.replace_feature(f)._sample_rows()[0] is first[0]
