@@ -116,6 +116,11 @@ class Muon(torch.optim.Optimizer):
             for p in params:
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon does not take sparse gradients")
+                if not p.is_cuda:                                        # refused before any state changes
+                    raise RuntimeError("orthogonalize runs on the GPU only (no CPU fallback): got a matrix on %s" % p.device)
+                if p.dtype not in _lib.DTYPE_CODE:
+                    raise TypeError("unsupported dtype %s" % p.dtype)
+            for p in params:
                 if "momentum_buffer" not in self.state[p]:
                     self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             grads = [p.grad for p in params]

@@ -200,6 +200,15 @@ def test_refusals_on_the_device(cuda_device):
         optim.orthogonalize([m, m.cpu()])
 
 
+def test_muon_refuses_before_it_changes_anything(cuda_device):
+    ok, bad = torch.nn.Parameter(torch.ones(4, 4, device=cuda_device)), torch.nn.Parameter(torch.ones(4, 4, device=cuda_device, dtype=torch.float64))
+    opt = optim.Muon([ok, bad])
+    ok.grad, bad.grad = torch.ones_like(ok), torch.ones_like(bad)
+    with pytest.raises(TypeError, match="float64"):
+        opt.step()
+    assert float((ok - 1).abs().max()) == 0 and not opt.state
+
+
 def test_training_step_with_all_of_them(cuda_device):
     """points -> dynamic voxel encoder (rows looked up) -> residual backbone with group norm -> dense -> backward -> Muon on the
     convolutions, AdamW on the rest: every parameter moves, the same way twice"""
