@@ -175,7 +175,9 @@ _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def act_name(module):
-    """the name `group_norm_act` has for an activation module, None if it has none"""
+    """the name `group_norm_act` has for an activation module, None if it has none or the module has hooks that want its own call"""
+    if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+        return None
     if type(module) is nn.ReLU:
         return "relu"
     if type(module) is nn.SiLU:

@@ -324,6 +324,49 @@ def test_sparse_module_and_sequential(cuda_device):
     assert x._sample_rows()[0].tolist() == [0, len(idx), len(idx), len(idx)]
 
 
+def test_hooks_of_an_activation_are_called(cuda_device):
+    feats, idx = _sites(cuda_device, 16)
+    seen, relu = [], torch.nn.ReLU()
+    seq = spconv.SparseSequential(spconv.SparseGroupNorm(4, 16).to(cuda_device), relu)
+    want = seq(spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)).features
+    relu.register_forward_hook(lambda m, i, o: seen.append(i[0]))
+    got = seq(spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)).features
+    assert len(seen) == 1 and float(seen[0].min()) < 0 and torch.equal(got, want)      # the clamp of the same fp32 values
+
+
+def test_sample_rows_follow_stream_and_capture(cuda_device):
+    feats, idx = _sites(cuda_device, 16, mixed=True)
+    gn = spconv.SparseGroupNorm(4, 16).to(cuda_device)
+    fresh = lambda i: gn(spconv.SparseConvTensor(feats, i, [8, 20, 20], 3)).features.detach()  # noqa: E731
+    x = spconv.SparseConvTensor(feats, idx.clone(), [8, 20, 20], 3)
+    want = [fresh(idx)]
+    swapped = idx.clone()
+    swapped[:, 0] = 2 - swapped[:, 0] + (swapped[:, 1] == 0).int()        # other frames, some rows in none
+    want.append(fresh(swapped))
+    first = x._sample_rows()[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert x._sample_rows()[0] is not first                           # this stream has not waited for that sort
+        other = gn(x).features.detach()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want[0])
+    for known in (False, True):                                           # captured before and after an eager call has listed the rows
+        x = spconv.SparseConvTensor(feats, idx.clone(), [8, 20, 20], 3)
+        if known:
+            gn(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = gn(x).features.detach()
+        assert torch.equal(gn(x).features.detach(), want[0])              # eager, before any replay
+        for k, indices in ((0, idx), (1, swapped), (0, idx), (1, swapped)):
+            x.indices.copy_(indices)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[k])
+            assert torch.equal(gn(x).features.detach(), want[k])
+
+
 def test_backbone_with_group_norm(cuda_device):
     torch.manual_seed(0)
     feats, idx = _sites(cuda_device, 5, batch=2)
