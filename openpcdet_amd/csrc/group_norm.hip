@@ -880,8 +880,8 @@ int check_args(int n, int c, int dtype, int samples, const int* offsets, int gro
     if (dtype < PVX_F32 || dtype > PVX_BF16 || param_dtype < PVX_F32 || param_dtype > PVX_BF16) return PVX_ERR_INVALID;
     if (act < PVX_ACT_NONE || act > PVX_ACT_GELU) return PVX_ERR_INVALID;
     if (!offsets && n % samples != 0) return PVX_ERR_INVALID;
-    // launches are indexed by (sample, group) and channel; positions, pieces and piece x channel products by 32 bits
-    if ((long long)samples * groups + c > 0x7fffffffLL || n > 0x7fffffff - (1 << 20) || c > (1 << 20)) return PVX_ERR_RANGE;
+    // the finishing kernels walk (sample, group) and channel in steps of a grid; positions, pieces and piece x channel products by 32 bits
+    if ((long long)samples * groups + c > 0x7fffffffLL - (1 << 16) || n > 0x7fffffff - (1 << 20) || c > (1 << 20)) return PVX_ERR_RANGE;
     return PVX_OK;
 }
 

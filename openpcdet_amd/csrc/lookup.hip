@@ -3,9 +3,9 @@
 //   out[i] = scale T[index[i]]                      (rows of zeros where index[i] is outside [0, m))
 //   dT[v]  = scale sum_{i : index[i] = v} dout[i]   (in ascending i; rows nobody looked up are zero)
 //
-// The gradient sorts the positions by index once (a stable counting sort by digits, below) and then every table row adds up its own
-// run of the list: sums in binary32, no atomics, the same bits on every run, and every row of dT is written exactly once.  Both
-// directions move bytes and nothing else: HBM bounds them, the launches at small sizes.
+// The gradient sorts the positions by index once (a stable counting sort by digits, below) and adds rows up in the order of the sorted
+// list: sums in binary32, no atomics, the same bits on every run.  Both directions move bytes and nothing else: HBM bounds them, the
+// launches at small sizes.
 #include "pvx_common.h"
 
 namespace {
