@@ -6,10 +6,11 @@
 // and with gz = dy act'(z), gx = w gz:
 //   db = sum gz, dw = sum gz xhat over all rows;   dx = (gx - mean gx - xhat mean(gx xhat)) / sqrt(v + eps);   dresidual = gz
 //
-// Ten to thirty flops per element: HBM bounds it.  A thread owns a chunk of four channels (fewer where c or an address does not allow
-// it; eight 16-bit ones cost so many registers that half as many waves were resident) and walks down the rows, as in batchnorm.hip; a workgroup owns a contiguous range of positions and takes the samples in
-// it one after the other, so ragged samples, empty ones and shared workgroups need no padding and no atomics: the piece of sample s in
-// workgroup k leaves its sums at index k + s (distinct, because later workgroups never see earlier samples).
+// Ten to thirty flops per element: HBM bounds it.  A thread owns a chunk of one to four channels and walks down the rows, as in
+// batchnorm.hip (eight 16-bit channels cost so many registers that half as many waves were resident); a workgroup owns a contiguous
+// range of positions and takes the samples in it one after the other, so ragged samples, empty ones and shared workgroups need no
+// padding and no atomics: the piece of sample s in workgroup k leaves its sums at index k + s (distinct, because later workgroups never
+// see earlier samples).
 // Sums are held in binary64: its adds run at the rate of binary32's here, and sum x^2 - (sum x)^2 / N keeps its digits.
 #include "pvx_common.h"
 
@@ -826,12 +827,12 @@ struct Shape {
     bool merged;                         // the apply kernels finish the sums
 };
 
-// elements of a thread's chunk: four, or two 16-bit ones, or one, as c and the addresses allow
+// elements of a thread's chunk that c and the addresses allow: four, two or one
 int chunk_of(int c, int dtype, std::initializer_list<const void*> ptrs) {
     const int es = dtype == PVX_F32 ? 4 : 2;
     uintptr_t low = 0;
     for (const void* p : ptrs) low |= (uintptr_t)p;
-    for (int v = 4; v > 1; v = es == 2 ? v / 2 : 1)
+    for (int v = 4; v > 1; v /= 2)
         if (c % v == 0 && low % ((uintptr_t)v * es) == 0) return v;
     return 1;
 }
@@ -848,6 +849,17 @@ Shape shape_of(int n, int c, int groups, int v) {
     s.blocks = PVX_CDIV(n, s.range);
     s.merged = s.tiles == 1 && (long long)s.blocks * groups <= kMergedSums;
     return s;
+}
+
+// Elements of a chunk in the forms of several launches.  Wide ones move more bytes an instruction, narrow ones have fewer sums to fold
+// at a range's end and shorter ranges.  Forward and backward, four / two / one of them: 30 000 x 64 bf16 46 / 36 / 33 us, 60 000 x 64
+// binary32 53 / 46 / 44, 117 301 x 64 bf16 56 / 50 / 52, 200 000 x 128 binary32 155 / 148 / 163, 400 000 x 128 bf16 157 / 169 / 235,
+// 520 013 x 128 binary32 398 / 483 / 508.  A row stays within one workgroup where it can: its groups are summed there.
+int narrowed(int v, int n, int c) {
+    const long long elements = (long long)n * c;
+    const int most = elements <= (1 << 22) ? 1 : (elements <= (1 << 25) ? 2 : 4);
+    while (v > most && 2 * (c / v) <= kBlk) v /= 2;
+    return v;
 }
 
 // workspace: one piece for each workgroup and one more for each sample that begins inside one (equal samples that fit the one-launch
@@ -875,6 +887,13 @@ int one_chunks(const Rows& rows, const Shape& sh, int groups, int most) {
     return u <= 4 ? 4 : (u <= most ? most : 0);
 }
 
+// the shape, and in `one` the rows of a thread in the one-launch form (0: the other form)
+Shape shape_for(const Rows& rows, int c, int groups, int v, int most, int& one) {
+    const Shape whole = shape_of(rows.n, c, groups, v);
+    one = one_chunks(rows, whole, groups, most);
+    return one ? whole : shape_of(rows.n, c, groups, narrowed(v, rows.n, c));
+}
+
 int check_args(int n, int c, int dtype, int samples, const int* offsets, int groups, int param_dtype, int act) {
     if (n < 0 || c <= 0 || samples <= 0 || groups <= 0 || c % groups != 0) return PVX_ERR_INVALID;
     if (dtype < PVX_F32 || dtype > PVX_BF16 || param_dtype < PVX_F32 || param_dtype > PVX_BF16) return PVX_ERR_INVALID;
@@ -890,7 +909,7 @@ dim3 finish_grid(long long results) { return dim3((unsigned)(results < 65536 ? r
 #define GN_DISPATCH(E, v, CALL)                                                            \
     do {                                                                                   \
         if (v == 4) { CALL(E, 4); }                                                        \
-        else if (sizeof(E) == 2 && v == 2) { CALL(E, (sizeof(E) == 2 ? 2 : 1)); }          \
+        else if (v == 2) { CALL(E, 2); }                                                   \
         else { CALL(E, 1); }                                                               \
     } while (0)
 #define GN_WITH_ACT(act, E, V, CALL)                                                       \
@@ -903,8 +922,8 @@ dim3 finish_grid(long long results) { return dim3((unsigned)(results < 65536 ? r
 
 template <typename E>
 int fwd_impl(const void* x, const Rows& rows, int c, int groups, const void* weight, const void* bias, int pd, float eps,
-             const void* residual, int act, void* y, float* mean, float* rstd, const Ws& ws, const Shape& sh, hipStream_t st) {
-    if (const int u = one_chunks(rows, sh, groups, kOneChunks)) {
+             const void* residual, int act, void* y, float* mean, float* rstd, const Ws& ws, const Shape& sh, int u, hipStream_t st) {
+    if (u) {
         const int blocks = rows.samples < kOneBlocks ? rows.samples : kOneBlocks;
         const dim3 one(blocks + (rows.offsets ? 1 : 0));
         const size_t lds = sizeof(double) * 2 * groups;
@@ -939,8 +958,8 @@ int fwd_impl(const void* x, const Rows& rows, int c, int groups, const void* wei
 template <typename E>
 int bwd_impl(const void* dy, const void* x, const void* residual, const Rows& rows, int c, int groups, const void* weight, const void* bias,
              int pd, const float* mean, const float* rstd, int act, void* dx, void* dres, void* dweight, void* dbias, const Ws& ws,
-             const Shape& sh, hipStream_t st) {
-    if (const int u = one_chunks(rows, sh, groups, kOneChunksBwd)) {
+             const Shape& sh, int u, hipStream_t st) {
+    if (u) {
         const int blocks = rows.samples < kOneBlocks ? rows.samples : kOneBlocks;
         const dim3 one(blocks + (rows.offsets ? 1 : 0));
         const size_t lds = sizeof(double) * 2 * groups;
@@ -1015,11 +1034,12 @@ extern "C" int pvx_group_norm_act_fwd(const void* x, int n, int c, int dtype, in
     const Ws ws = carve(cv, c, samples, groups, pieces_cap(n, c, samples, offsets != nullptr));
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const Rows rows{offsets, order, n, samples, offsets ? 0 : n / samples};
-    const Shape sh = shape_of(n, c, groups, chunk_of(c, dtype, {x, residual, y}));
+    int one;
+    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {x, residual, y}), kOneChunks, one);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == PVX_F32) return fwd_impl<float>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, st);
-    if (dtype == PVX_F16) return fwd_impl<_Float16>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, st);
-    return fwd_impl<__bf16>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, st);
+    if (dtype == PVX_F32) return fwd_impl<float>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, one, st);
+    if (dtype == PVX_F16) return fwd_impl<_Float16>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, one, st);
+    return fwd_impl<__bf16>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, one, st);
 }
 
 extern "C" int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, int n, int c, int dtype, int samples,
@@ -1040,8 +1060,9 @@ extern "C" int pvx_group_norm_act_bwd(const void* dy, const void* x, const void*
     const Ws ws = carve(cv, c, samples, groups, pieces_cap(n, c, samples, offsets != nullptr));
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const Rows rows{offsets, order, n, samples, offsets ? 0 : n / samples};
-    const Shape sh = shape_of(n, c, groups, chunk_of(c, dtype, {dy, x, residual, dx, dresidual}));
-    if (dtype == PVX_F32) return bwd_impl<float>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, st);
-    if (dtype == PVX_F16) return bwd_impl<_Float16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, st);
-    return bwd_impl<__bf16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, st);
+    int one;
+    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {dy, x, residual, dx, dresidual}), kOneChunksBwd, one);
+    if (dtype == PVX_F32) return bwd_impl<float>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
+    if (dtype == PVX_F16) return bwd_impl<_Float16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
+    return bwd_impl<__bf16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
 }

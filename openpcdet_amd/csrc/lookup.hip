@@ -35,10 +35,12 @@ __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__
     __shared__ int cnt[kWaves][kDigits];
     __shared__ int wsum[kDigits / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rounds = PVX_CDIV(n, kOneBlk), first = wave * rounds * 64 + lane;      // a wave's keys lie together, on all waves alike
     int key[kOneKeys], idx[kOneKeys], at[kOneKeys];
 #pragma unroll
     for (int r = 0; r < kOneKeys; r++) {
-        const int i = (wave * kOneKeys + r) * 64 + lane;
+        const int i = first + r * 64;
+        if (r >= rounds) break;
         idx[r] = i;
         key[r] = i < n ? key_of<I>(index[i], m) : m;
     }
@@ -48,7 +50,8 @@ __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kOneKeys; r++) {
-            const bool on = (wave * kOneKeys + r) * 64 + lane < n;
+            if (r >= rounds) break;
+            const bool on = first + r * 64 < n;
             const int d = (key[r] >> shift) & ((1 << bits) - 1);
             const unsigned long long mask = same_digit(d, bits, on);
             const int before = __popcll(mask & ((1ull << lane) - 1ull));
@@ -76,7 +79,7 @@ __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kOneKeys; r++) {
-            if ((wave * kOneKeys + r) * 64 + lane < n) {
+            if (r < rounds && first + r * 64 < n) {
                 const int to = cnt[wave][(key[r] >> shift) & ((1 << bits) - 1)] + at[r];
                 skey[to] = key[r];
                 sidx[to] = idx[r];
@@ -85,15 +88,15 @@ __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kOneKeys; r++) {
-            const int i = (wave * kOneKeys + r) * 64 + lane;
-            if (i < n) { key[r] = skey[i]; idx[r] = sidx[i]; }
+            const int i = first + r * 64;
+            if (r < rounds && i < n) { key[r] = skey[i]; idx[r] = sidx[i]; }
         }
         __syncthreads();
     }
 #pragma unroll
     for (int r = 0; r < kOneKeys; r++) {
-        const int i = (wave * kOneKeys + r) * 64 + lane;
-        if (i < n) { order[i] = idx[r]; keys_out[i] = key[r]; }
+        const int i = first + r * 64;
+        if (r < rounds && i < n) { order[i] = idx[r]; keys_out[i] = key[r]; }
     }
     if (offsets) {                       // skey holds the sorted keys (total_bits >= 1: at least one pass ran)
         for (int v = threadIdx.x; v <= m; v += kOneBlk) {
@@ -308,9 +311,9 @@ __global__ __launch_bounds__(kBlk) void lookup_kernel(const E* __restrict__ tabl
 // leaves what the block holds of it: the run that comes in from the left (or is the whole block) as the block's head, the one that goes on
 // to the right as its tail.  Blocks of kFan whole heads, and once more, are added up where they carry one key; then the block in which a
 // crossing run begins joins its tail, whole blocks by the largest that fit, and the last head: at most 2 kWorth + n / kFan^3 steps,
-// whatever share of the list the row has.  (A level is made where the one before has kWorth blocks.)  All work is in proportion to
-// the list, so the table is cleared beforehand; a walk through each row's run by its offsets instead took 1.7 times as long where
-// the runs' lengths differ much.
+// whatever share of the list the row has.  (A level is made where the one before has kWorth blocks: 2 us where no run is long, 240 000
+// keys 63 -> 64 us; 1 048 579 skewed keys 337 -> 264.)  All work is in proportion to the list, so the table is cleared beforehand; a
+// walk through each row's run by its offsets instead took 1.7 times as long where the runs' lengths differ much.
 constexpr int kFan = 64, kFanLog = 6, kLevels = 3, kWorth = 256;
 
 template <typename E, int V> __device__ __forceinline__ void store_row(E* dtable, long long at, const float (&acc)[V], float scale) {
@@ -469,7 +472,8 @@ int bits_of(int m) {                     // bits of the keys 0 .. m (m >= 1)
     return b;
 }
 
-// keys of a thread in a pass: tiles of 1024 keys while they are few, so that the chip has work; of 2048 where their counts would weigh
+// Keys of a thread in a pass: tiles of 1024 keys while they are few, so that the chip has work; of 2048 where their counts would weigh
+// (lookup and gradient, four / eight: 240 000 keys 64 / 74 us, 1 048 579 keys 268 / 264).
 int rounds_of(int n) { return n <= (1 << 19) ? 4 : 8; }
 int tiles_of(int n) { return (int)PVX_CDIV((long long)n, (long long)rounds_of(n) * kBlk); }
 
@@ -483,7 +487,9 @@ template <typename C> void carve_sort(C& cv, int n, SortWs* w) {
     w->totals = cv.template take<int>(many ? (size_t)1 << kMaxBits : 0);
 }
 
-constexpr int kOwnScan = 1 << 14;        // counts that every scatter workgroup adds up itself rather than leave them to a launch between
+// Counts that every scatter workgroup adds up itself rather than leave them to a launch between: the GPU's time is the same (49 us for
+// 30 000 keys either way) and the host has two launches fewer; more counts cost time (240 000 keys 64 -> 80 us).
+constexpr int kOwnScan = 1 << 14;
 
 template <typename I>
 int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const SortWs& w, int2* out, int* keys, int* order, hipStream_t st) {
@@ -608,10 +614,12 @@ int grad_dispatch(const void* dout, const int* order, const int* keys, int n, in
     LK_DISPATCH(E, v, LK_GRAD);
 }
 
+// A thread takes four rows where there are rows enough (four / one: 1000 x 64 binary32 5.9 / 4.6 us, 20 000 x 64 5.2 / 5.5, 60 000 x 32
+// 5.4 / 6.1, 240 000 x 32 10 / 13, 1 048 579 x 128 bf16 80 / 107).
 template <typename E, int V>
 int lookup_impl(const E* table, const void* index, int index64, int n, int m, int width, float scale, E* out, hipStream_t st) {
     const int ch = width / V;
-    const dim3 grid = grid_for(n, ch, n >= 65536 ? 4 : 1);
+    const dim3 grid = grid_for(n, ch, n >= 16384 ? 4 : 1);
     if (index64) hipLaunchKernelGGL((lookup_kernel<E, V, long long>), grid, dim3(kBlk), 0, st, table, (const long long*)index, n, ch, m, scale, out);
     else hipLaunchKernelGGL((lookup_kernel<E, V, int>), grid, dim3(kBlk), 0, st, table, (const int*)index, n, ch, m, scale, out);
     PVX_CHECK_LAUNCH();
