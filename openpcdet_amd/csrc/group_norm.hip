@@ -18,12 +18,15 @@ namespace {
 
 constexpr int kBlk = 512, kWaves = kBlk / 64;
 constexpr int kResident = 4;             // waves of a SIMD that the registers leave room for
-constexpr int kTargetBlocks = 256 * 4 * kResident / kWaves;      // ranges of positions: all of them resident together, no second turn
-constexpr int kMergedSums = 8192;        // pieces x groups that the apply kernels add up for themselves
+// Ranges of positions: all of them resident together, no second turn (with half / twice as many 117 301 x 64 bf16 takes 63 / 78 us
+// instead of 65, 106 032 x 96 f16 forward 31 / 34 instead of 25, 520 013 x 128 binary32 453 / 445 instead of 410; chunks of four).
+constexpr int kTargetBlocks = 256 * 4 * kResident / kWaves;
+// Pieces x groups that the apply kernels add up for themselves rather than leave them to a launch between: the GPU's time is the same
+// (117 301 x 64 bf16 forward and backward 65.1 us, 64.5 with that launch), the host's is shorter by two launches.
+constexpr int kMergedSums = 8192;
 // rows of a thread whose loads are on their way together
 template <typename E, int V> constexpr int kAhead = sizeof(E) * V == 16 ? 2 : 4;
-constexpr int kOneChunks = 16, kOneChunksBwd = 8;       // chunks a thread of the one-launch form holds (the backward: of two tensors)
-constexpr int kOneBlocks = 2048;         // workgroups of that form: more samples than this are taken in turns
+constexpr int kOneChunks = 4, kOneSamples = 512;        // the one-launch form: rows of a thread, and samples
 
 template <typename E, int V> struct alignas(sizeof(E) * V) Pack { E e[V]; };
 
@@ -479,13 +482,15 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_sums_kernel(const E* _
 __device__ __forceinline__ void channel_finish(const double* partial, const Rows& rows, int c, int range, int cc, int pd, void* dweight, void* dbias,
                                                double* red) {
     double a = 0.0, b = 0.0;
-    // few samples: the threads stride over a sample's pieces; many: over the samples
-    const bool many = rows.samples >= kBlk;
-    for (int s = many ? threadIdx.x : 0; s < rows.samples; s += many ? kBlk : 1) {
+    // as many lanes a sample as it has pieces on average, so that the samples are not walked one after the other
+    const int average = PVX_CDIV(PVX_CDIV(rows.n, range), rows.samples) + 1;
+    int lanes = 1;
+    while (lanes < average && lanes < kBlk) lanes <<= 1;
+    for (int s = threadIdx.x / lanes; s < rows.samples; s += kBlk / lanes) {
         const int lo = rows.begin(s), hi = rows.begin(s + 1);
         if (hi <= lo) continue;
         const int k0 = lo / range, pieces = (hi - 1) / range - k0 + 1;
-        for (int i = many ? 0 : threadIdx.x; i < pieces; i += many ? 1 : kBlk) {
+        for (int i = threadIdx.x & (lanes - 1); i < pieces; i += lanes) {
             const double2 q = *reinterpret_cast<const double2*>(partial + ((size_t)(k0 + s + i) * c + cc) * 2);
             a += q.x;
             b += q.y;
@@ -618,9 +623,11 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_apply_kernel(const E* 
     }
 }
 
-// One launch: a workgroup holds one sample's rows in registers (at most kOneChunks chunks a thread), so x is read once and nothing but
-// the statistics goes through memory.  Taken where every sample is known to fit: latency is what such calls cost (three launches
-// otherwise).  blockIdx.x == samples: the positions of no sample.
+// One launch: a workgroup holds one sample's rows in registers (kOneChunks chunks a thread), so x is read once and nothing but the
+// statistics goes through memory.  Taken where every sample is known to fit and all workgroups run at a time: latency is what such calls
+// cost.  Against the form of several launches, forward / forward and backward: 128 rows x 64 binary32 8.2 / 16.5 us and 9.5 / 17.3, 256
+// samples of 30 rows 7.4 / 18 and 14 / 28; but 1000 samples of 120 rows 19 / 60 and 20 / 47, and with sixteen rows a thread (eight
+// backward) 510 rows 13 / 22 and 9.5 / 18.  blockIdx.x == samples: the positions of no sample.
 template <typename E, int V>
 __device__ __forceinline__ void zero_uncovered(const Place& t, const Rows& rows, int c, E* a, E* b) {
     if (!t.on) return;
@@ -635,83 +642,82 @@ __device__ __forceinline__ void zero_uncovered(const Place& t, const Rows& rows,
     }
 }
 
-template <typename E, int V, int U>
+template <typename E, int V>
 __global__ __launch_bounds__(kBlk) void gn_one_kernel(const E* __restrict__ x, const E* __restrict__ residual, Rows rows, int c, int groups,
                                                        const void* __restrict__ weight, const void* __restrict__ bias, int pd, float eps,
                                                        int act, E* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     __shared__ double red[2 * kBlk * (V + 1)];
     extern __shared__ double per_group[];                // [groups][2]
     const Place t = place<V>(c);
-    const int cpg = c / groups, blocks = gridDim.x - (rows.offsets ? 1 : 0);
-    if ((int)blockIdx.x == blocks) { zero_uncovered<E, V>(t, rows, c, y, (E*)nullptr); return; }
+    constexpr int U = kOneChunks;
+    const int cpg = c / groups, s = blockIdx.x;
+    if (s == rows.samples) { zero_uncovered<E, V>(t, rows, c, y, (E*)nullptr); return; }
     float w[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
         w[j] = t.on ? load_param(weight, pd, t.chunk * V + j, 1.f) : 0.f;
         b[j] = t.on ? load_param(bias, pd, t.chunk * V + j, 0.f) : 0.f;
     }
-    for (int s = blockIdx.x; s < rows.samples; s += blocks) {
-        const int lo = rows.begin(s), hi = min(rows.begin(s + 1), lo + U * t.rpb);
-        float v[U][V];
-        double s0[V], s1[V];
+    const int lo = rows.begin(s), hi = min(rows.begin(s + 1), lo + U * t.rpb);
+    float v[U][V];
+    double s0[V], s1[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) { s0[j] = 0; s1[j] = 0; }
+    for (int j = 0; j < V; j++) { s0[j] = 0; s1[j] = 0; }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int p = lo + t.r_in + u * t.rpb;
-            const int row = t.on && p < hi ? rows.row(p) : -1;
+    for (int u = 0; u < U; u++) {
+        const int p = lo + t.r_in + u * t.rpb;
+        const int row = t.on && p < hi ? rows.row(p) : -1;
 #pragma unroll
-            for (int j = 0; j < V; j++) v[u][j] = 0.f;
-            if (row >= 0) load_pack<E, V>(x + (size_t)row * c + t.chunk * V, v[u]);
-        }
+        for (int j = 0; j < V; j++) v[u][j] = 0.f;
+        if (row >= 0) load_pack<E, V>(x + (size_t)row * c + t.chunk * V, v[u]);
+    }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
+    for (int u = 0; u < U; u++) {
 #pragma unroll
-            for (int j = 0; j < V; j++) { const double d = v[u][j]; s0[j] += d; s1[j] = fma(d, d, s1[j]); }
-        }
-        fold_rows<V>(s0, s1, t, red);
-        group_sums<V>(c, groups, red, per_group);
-        for (int g = threadIdx.x; g < groups; g += kBlk) {
-            const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
-            const double mu = per_group[2 * g] / count;
-            double var = per_group[2 * g + 1] / count - mu * mu;
-            if (var < 0.0) var = 0.0;
-            const double rs = 1.0 / sqrt(var + (double)eps);
-            per_group[2 * g] = mu;
-            per_group[2 * g + 1] = rs;
-            mean[(size_t)s * groups + g] = (float)mu;
-            rstd[(size_t)s * groups + g] = (float)rs;
-        }
-        __syncthreads();
-        if (!t.on) continue;
-        float mu[V], rs[V];
+        for (int j = 0; j < V; j++) { const double d = v[u][j]; s0[j] += d; s1[j] = fma(d, d, s1[j]); }
+    }
+    fold_rows<V>(s0, s1, t, red);
+    group_sums<V>(c, groups, red, per_group);
+    for (int g = threadIdx.x; g < groups; g += kBlk) {
+        const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
+        const double mu = per_group[2 * g] / count;
+        double var = per_group[2 * g + 1] / count - mu * mu;
+        if (var < 0.0) var = 0.0;
+        const double rs = 1.0 / sqrt(var + (double)eps);
+        per_group[2 * g] = mu;
+        per_group[2 * g + 1] = rs;
+        mean[(size_t)s * groups + g] = (float)mu;
+        rstd[(size_t)s * groups + g] = (float)rs;
+    }
+    __syncthreads();
+    if (!t.on) return;
+    float mu[V], rs[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        const int g = (t.chunk * V + j) / cpg;
+        mu[j] = (float)per_group[2 * g];
+        rs[j] = (float)per_group[2 * g + 1];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int p = lo + t.r_in + u * t.rpb;
+        const int row = p < hi ? rows.row(p) : -1;
+        if (row < 0) continue;
+        const size_t off = (size_t)row * c + t.chunk * V;
+        float r[V];
+        if (residual) load_pack<E, V>(residual + off, r);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const int g = (t.chunk * V + j) / cpg;
-            mu[j] = (float)per_group[2 * g];
-            rs[j] = (float)per_group[2 * g + 1];
+            float z = (v[u][j] - mu[j]) * rs[j] * w[j] + b[j];
+            if (residual) z += r[j];
+            v[u][j] = act_of(z, act);
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int p = lo + t.r_in + u * t.rpb;
-            const int row = p < hi ? rows.row(p) : -1;
-            if (row < 0) continue;
-            const size_t off = (size_t)row * c + t.chunk * V;
-            float r[V];
-            if (residual) load_pack<E, V>(residual + off, r);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                float z = (v[u][j] - mu[j]) * rs[j] * w[j] + b[j];
-                if (residual) z += r[j];
-                v[u][j] = act_of(z, act);
-            }
-            store_pack<E, V>(y + off, v[u]);
-        }
+        store_pack<E, V>(y + off, v[u]);
     }
 }
 
-// the backward of the same; a workgroup adds dw and db up over its samples and leaves them in partial[workgroup][2][c]
-template <typename E, int V, int U>
+// the backward of the same; a workgroup leaves its sample's share of db and dw in partial[sample][2][c]
+template <typename E, int V>
 __global__ __launch_bounds__(kBlk) void gn_bwd_one_kernel(const E* __restrict__ dy, const E* __restrict__ x, const E* __restrict__ residual,
                                                            Rows rows, int c, int groups, const void* __restrict__ weight,
                                                            const void* __restrict__ bias, int pd, const float* __restrict__ mean,
@@ -720,87 +726,81 @@ __global__ __launch_bounds__(kBlk) void gn_bwd_one_kernel(const E* __restrict__ 
     __shared__ double red[2 * kBlk * (V + 1)];
     extern __shared__ double per_group[];
     const Place t = place<V>(c);
-    const int cpg = c / groups, blocks = gridDim.x - (rows.offsets ? 1 : 0);
-    if ((int)blockIdx.x == blocks) { zero_uncovered<E, V>(t, rows, c, dx, dres); return; }
-    double db[V], dw[V];
+    constexpr int U = kOneChunks;
+    const int cpg = c / groups, s = blockIdx.x;
+    if (s == rows.samples) { zero_uncovered<E, V>(t, rows, c, dx, dres); return; }
+    const int lo = rows.begin(s), hi = min(rows.begin(s + 1), lo + U * t.rpb);
+    float xh[U][V], gz[U][V];
+    Chan<V> k;
 #pragma unroll
-    for (int j = 0; j < V; j++) { db[j] = 0; dw[j] = 0; }
-    for (int s = blockIdx.x; s < rows.samples; s += blocks) {
-        const int lo = rows.begin(s), hi = min(rows.begin(s + 1), lo + U * t.rpb);
-        float xh[U][V], gz[U][V];
-        Chan<V> k;
+    for (int j = 0; j < V; j++) { k.mu[j] = 0.f; k.rs[j] = 0.f; k.w[j] = 0.f; k.b[j] = 0.f; }
+    if (t.on) load_chan<V>(k, t.chunk * V, s, groups, cpg, weight, bias, pd, mean, rstd);
+    double s0[V], s1[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) { k.mu[j] = 0.f; k.rs[j] = 0.f; k.w[j] = 0.f; k.b[j] = 0.f; }
-        if (t.on) load_chan<V>(k, t.chunk * V, s, groups, cpg, weight, bias, pd, mean, rstd);
-        double s0[V], s1[V];
+    for (int j = 0; j < V; j++) { s0[j] = 0; s1[j] = 0; }
 #pragma unroll
-        for (int j = 0; j < V; j++) { s0[j] = 0; s1[j] = 0; }
+    for (int u = 0; u < U; u++) {
+        const int p = lo + t.r_in + u * t.rpb;
+        const int row = t.on && p < hi ? rows.row(p) : -1;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int p = lo + t.r_in + u * t.rpb;
-            const int row = t.on && p < hi ? rows.row(p) : -1;
-#pragma unroll
-            for (int j = 0; j < V; j++) { xh[u][j] = 0.f; gz[u][j] = 0.f; }
-            if (row < 0) continue;
-            const size_t off = (size_t)row * c + t.chunk * V;
-            float r[V];
-            load_pack<E, V>(dy + off, gz[u]);
-            load_pack<E, V>(x + off, xh[u]);
-            if (residual) load_pack<E, V>(residual + off, r);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                xh[u][j] = (xh[u][j] - k.mu[j]) * k.rs[j];
-                float z = xh[u][j] * k.w[j] + k.b[j];
-                if (residual) z += r[j];
-                gz[u][j] *= slope_of(z, act);
-                s0[j] += (double)gz[u][j];
-                s1[j] = fma((double)gz[u][j], (double)xh[u][j], s1[j]);
-            }
-        }
-        fold_rows<V>(s0, s1, t, red);
-        if (t.on && t.r_in == 0) {
-            double(*r0)[V + 1] = reinterpret_cast<double(*)[V + 1]>(red);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                db[j] += s0[j];
-                dw[j] += s1[j];
-                r0[threadIdx.x][j] = s0[j] * (double)k.w[j];     // the groups' sums take w gz
-                r0[kBlk + threadIdx.x][j] = s1[j] * (double)k.w[j];
-            }
-        }
-        group_sums<V>(c, groups, red, per_group);
-        if (!t.on) continue;
-        const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
-        float a[V], b[V];
+        for (int j = 0; j < V; j++) { xh[u][j] = 0.f; gz[u][j] = 0.f; }
+        if (row < 0) continue;
+        const size_t off = (size_t)row * c + t.chunk * V;
+        float r[V];
+        load_pack<E, V>(dy + off, gz[u]);
+        load_pack<E, V>(x + off, xh[u]);
+        if (residual) load_pack<E, V>(residual + off, r);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const int g = (t.chunk * V + j) / cpg;
-            a[j] = (float)(per_group[2 * g] / count);
-            b[j] = (float)(per_group[2 * g + 1] / count);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int p = lo + t.r_in + u * t.rpb;
-            const int row = p < hi ? rows.row(p) : -1;
-            if (row < 0) continue;
-            const size_t off = (size_t)row * c + t.chunk * V;
-            float o[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) o[j] = k.rs[j] * (gz[u][j] * k.w[j] - a[j] - xh[u][j] * b[j]);
-            store_pack<E, V>(dx + off, o);
-            if (dres) store_pack<E, V>(dres + off, gz[u]);
+            xh[u][j] = (xh[u][j] - k.mu[j]) * k.rs[j];
+            float z = xh[u][j] * k.w[j] + k.b[j];
+            if (residual) z += r[j];
+            gz[u][j] *= slope_of(z, act);
+            s0[j] += (double)gz[u][j];
+            s1[j] = fma((double)gz[u][j], (double)xh[u][j], s1[j]);
         }
     }
+    fold_rows<V>(s0, s1, t, red);
     if (t.on && t.r_in == 0) {
-        double* out = partial + (size_t)blockIdx.x * 2 * c + t.chunk * V;
+        double(*r0)[V + 1] = reinterpret_cast<double(*)[V + 1]>(red);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            if (blocks == 1) {
-                if (dbias) store_param(dbias, pd, t.chunk * V + j, db[j]);
-                if (dweight) store_param(dweight, pd, t.chunk * V + j, dw[j]);
+            r0[threadIdx.x][j] = s0[j] * (double)k.w[j];     // the groups' sums take w gz
+            r0[kBlk + threadIdx.x][j] = s1[j] * (double)k.w[j];
+        }
+    }
+    group_sums<V>(c, groups, red, per_group);
+    if (!t.on) return;
+    const double count = hi > lo ? (double)(hi - lo) * cpg : 1.0;
+    float a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        const int g = (t.chunk * V + j) / cpg;
+        a[j] = (float)(per_group[2 * g] / count);
+        b[j] = (float)(per_group[2 * g + 1] / count);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int p = lo + t.r_in + u * t.rpb;
+        const int row = p < hi ? rows.row(p) : -1;
+        if (row < 0) continue;
+        const size_t off = (size_t)row * c + t.chunk * V;
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) o[j] = k.rs[j] * (gz[u][j] * k.w[j] - a[j] - xh[u][j] * b[j]);
+        store_pack<E, V>(dx + off, o);
+        if (dres) store_pack<E, V>(dres + off, gz[u]);
+    }
+    if (t.r_in == 0) {
+        double* out = partial + (size_t)s * 2 * c + t.chunk * V;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            if (rows.samples == 1) {
+                if (dbias) store_param(dbias, pd, t.chunk * V + j, s0[j]);
+                if (dweight) store_param(dweight, pd, t.chunk * V + j, s1[j]);
             } else {
-                out[j] = db[j];
-                out[c + j] = dw[j];
+                out[j] = s0[j];
+                out[c + j] = s1[j];
             }
         }
     }
@@ -863,9 +863,9 @@ int narrowed(int v, int n, int c) {
 }
 
 // workspace: one piece for each workgroup and one more for each sample that begins inside one (equal samples that fit the one-launch
-// form whatever the alignment need its workgroups only), and the backward's two means per (sample, group)
+// form whatever the alignment need one each), and the backward's two means per (sample, group)
 size_t pieces_cap(int n, int c, int samples, bool ragged) {
-    if (!ragged && c <= kBlk && n / samples <= kOneChunksBwd * (kBlk / c)) return samples < kOneBlocks ? samples : kOneBlocks;
+    if (!ragged && c <= kBlk && samples <= kOneSamples && n / samples <= kOneChunks * (kBlk / c)) return samples;
     return (size_t)(n < kTargetBlocks ? n : kTargetBlocks) + samples;
 }
 
@@ -880,17 +880,11 @@ template <typename C> Ws carve(C& cv, int c, int samples, int groups, size_t pie
     return w;
 }
 
-// rows of a thread when a workgroup takes a whole sample: 4 or `most`; 0: some sample may not fit
-int one_chunks(const Rows& rows, const Shape& sh, int groups, int most) {
-    if (sh.tiles != 1 || groups > 1024) return 0;
-    const int u = PVX_CDIV(rows.offsets ? rows.n : rows.each, sh.rpb);
-    return u <= 4 ? 4 : (u <= most ? most : 0);
-}
-
-// the shape, and in `one` the rows of a thread in the one-launch form (0: the other form)
-Shape shape_for(const Rows& rows, int c, int groups, int v, int most, int& one) {
+// the shape, and in `one` whether a workgroup takes a whole sample
+Shape shape_for(const Rows& rows, int c, int groups, int v, bool& one) {
     const Shape whole = shape_of(rows.n, c, groups, v);
-    one = one_chunks(rows, whole, groups, most);
+    one = whole.tiles == 1 && groups <= 1024 && rows.samples <= kOneSamples
+          && PVX_CDIV(rows.offsets ? rows.n : rows.each, whole.rpb) <= kOneChunks;
     return one ? whole : shape_of(rows.n, c, groups, narrowed(v, rows.n, c));
 }
 
@@ -922,16 +916,12 @@ dim3 finish_grid(long long results) { return dim3((unsigned)(results < 65536 ? r
 
 template <typename E>
 int fwd_impl(const void* x, const Rows& rows, int c, int groups, const void* weight, const void* bias, int pd, float eps,
-             const void* residual, int act, void* y, float* mean, float* rstd, const Ws& ws, const Shape& sh, int u, hipStream_t st) {
-    if (u) {
-        const int blocks = rows.samples < kOneBlocks ? rows.samples : kOneBlocks;
-        const dim3 one(blocks + (rows.offsets ? 1 : 0));
+             const void* residual, int act, void* y, float* mean, float* rstd, const Ws& ws, const Shape& sh, bool is_one, hipStream_t st) {
+    if (is_one) {
+        const dim3 one(rows.samples + (rows.offsets ? 1 : 0));
         const size_t lds = sizeof(double) * 2 * groups;
-#define GN_ONE(E, V)                                                                                                                        \
-        if (u == 4) hipLaunchKernelGGL((gn_one_kernel<E, V, 4>), one, dim3(kBlk), lds, st, (const E*)x, (const E*)residual, rows, c, groups, \
-                                       weight, bias, pd, eps, act, (E*)y, mean, rstd);                                                      \
-        else hipLaunchKernelGGL((gn_one_kernel<E, V, kOneChunks>), one, dim3(kBlk), lds, st, (const E*)x, (const E*)residual, rows, c,       \
-                                groups, weight, bias, pd, eps, act, (E*)y, mean, rstd)
+#define GN_ONE(E, V) hipLaunchKernelGGL((gn_one_kernel<E, V>), one, dim3(kBlk), lds, st, (const E*)x, (const E*)residual, rows, c, groups, \
+                                        weight, bias, pd, eps, act, (E*)y, mean, rstd)
         GN_DISPATCH(E, sh.v, GN_ONE);
         PVX_CHECK_LAUNCH();
         return PVX_OK;
@@ -958,22 +948,17 @@ int fwd_impl(const void* x, const Rows& rows, int c, int groups, const void* wei
 template <typename E>
 int bwd_impl(const void* dy, const void* x, const void* residual, const Rows& rows, int c, int groups, const void* weight, const void* bias,
              int pd, const float* mean, const float* rstd, int act, void* dx, void* dres, void* dweight, void* dbias, const Ws& ws,
-             const Shape& sh, int u, hipStream_t st) {
-    if (u) {
-        const int blocks = rows.samples < kOneBlocks ? rows.samples : kOneBlocks;
-        const dim3 one(blocks + (rows.offsets ? 1 : 0));
+             const Shape& sh, bool is_one, hipStream_t st) {
+    if (is_one) {
+        const dim3 one(rows.samples + (rows.offsets ? 1 : 0));
         const size_t lds = sizeof(double) * 2 * groups;
-#define GN_BONE(E, V)                                                                                                                    \
-        if (u == 4) hipLaunchKernelGGL((gn_bwd_one_kernel<E, V, 4>), one, dim3(kBlk), lds, st, (const E*)dy, (const E*)x,                \
-                                       (const E*)residual, rows, c, groups, weight, bias, pd, mean, rstd, act, (E*)dx, (E*)dres, dweight, \
-                                       dbias, ws.partial);                                                                               \
-        else hipLaunchKernelGGL((gn_bwd_one_kernel<E, V, kOneChunksBwd>), one, dim3(kBlk), lds, st, (const E*)dy, (const E*)x,               \
-                                (const E*)residual, rows, c, groups, weight, bias, pd, mean, rstd, act, (E*)dx, (E*)dres, dweight, dbias, \
-                                ws.partial)
+#define GN_BONE(E, V) hipLaunchKernelGGL((gn_bwd_one_kernel<E, V>), one, dim3(kBlk), lds, st, (const E*)dy, (const E*)x,                \
+                                         (const E*)residual, rows, c, groups, weight, bias, pd, mean, rstd, act, (E*)dx, (E*)dres,     \
+                                         dweight, dbias, ws.partial)
         GN_DISPATCH(E, sh.v, GN_BONE);
         PVX_CHECK_LAUNCH();
-        if (blocks > 1 && (dweight || dbias)) {
-            hipLaunchKernelGGL(gn_bwd_channels_kernel, dim3(c), dim3(64), 0, st, ws.partial, blocks, c, pd, dweight, dbias);
+        if (rows.samples > 1 && (dweight || dbias)) {
+            hipLaunchKernelGGL(gn_bwd_channels_kernel, dim3(c), dim3(64), 0, st, ws.partial, rows.samples, c, pd, dweight, dbias);
             PVX_CHECK_LAUNCH();
         }
         return PVX_OK;
@@ -1034,8 +1019,8 @@ extern "C" int pvx_group_norm_act_fwd(const void* x, int n, int c, int dtype, in
     const Ws ws = carve(cv, c, samples, groups, pieces_cap(n, c, samples, offsets != nullptr));
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const Rows rows{offsets, order, n, samples, offsets ? 0 : n / samples};
-    int one;
-    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {x, residual, y}), kOneChunks, one);
+    bool one;
+    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {x, residual, y}), one);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == PVX_F32) return fwd_impl<float>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, one, st);
     if (dtype == PVX_F16) return fwd_impl<_Float16>(x, rows, c, groups, weight, bias, param_dtype, eps, residual, act, y, save_mean, save_rstd, ws, sh, one, st);
@@ -1060,8 +1045,8 @@ extern "C" int pvx_group_norm_act_bwd(const void* dy, const void* x, const void*
     const Ws ws = carve(cv, c, samples, groups, pieces_cap(n, c, samples, offsets != nullptr));
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const Rows rows{offsets, order, n, samples, offsets ? 0 : n / samples};
-    int one;
-    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {dy, x, residual, dx, dresidual}), kOneChunksBwd, one);
+    bool one;
+    const Shape sh = shape_for(rows, c, groups, chunk_of(c, dtype, {dy, x, residual, dx, dresidual}), one);
     if (dtype == PVX_F32) return bwd_impl<float>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
     if (dtype == PVX_F16) return bwd_impl<_Float16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
     return bwd_impl<__bf16>(dy, x, residual, rows, c, groups, weight, bias, param_dtype, save_mean, save_rstd, act, dx, dresidual, dweight, dbias, ws, sh, one, st);
