@@ -15,6 +15,10 @@
 // A and B are symmetric: only tiles on or below the diagonal are computed, and both factors of A = X X^T and A A are read along k.
 // B X reads X by rows of k: its fragments come out of LDS transposed (ds_read_b64_tr_b16).  Buffers are padded with zeros to whole
 // tiles, which the products reproduce.
+//
+// Wide matrices are bound by the matrix cores: 2048 x 4096 takes 1167 us for 926 Gflop in f16 (three products each), 794 Tflop/s, where
+// the best library product of bf16 reaches 1054 (8192^3).  Few or narrow ones are bound by their launches, five a step: a backbone's
+// 21 layers take 172 us, of which the products are 23 a step.
 #include "pvx_common.h"
 
 #include <math.h>
@@ -30,8 +34,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-constexpr int kBlk = 256, kBK = 32, kMaxMats = 64, kNormBlocks = 256, kNormChunk = 8192, kMaxSteps = 64, kWhole = 256;
-
+constexpr int kBlk = 256, kBK = 32, kMaxMats = 64, kNormBlocks = 256, kNormChunk = 8192, kMaxSteps = 64;
+// Rows up to which lo lo is added too.  There sums are short and a dropped 2^-24 is seen against binary32's own rounding; it costs 1 %
+// (256 x 2304 147 us, 145 without).  Longer sums hide it, and it costs 14 % (2048 x 4096 1333 us, 1167 without).
+constexpr int kWhole = 256;
 
 struct Mat {
     const void* in;
@@ -298,7 +304,8 @@ template <typename E, int T, int MODE>
 __global__ __launch_bounds__(kBlk) void ns_product_kernel(Table t, char* ws, int step, int last) {
     constexpr int N = T / 64;                            // staging rounds; 32 x 32 blocks of a wave along each side
     constexpr int kRow = 2 * T + 32;                     // bytes of a row of k
-    constexpr int kD = T == 128 ? 1 : 2;                 // buffers: three workgroups of one, four of two on a CU (measured: the better ones)
+    // LDS buffers: three workgroups on a CU with one of 128, four with two of 64 (one / two: 2048 x 4096 1167 / 1230 us, 512 x 2304 204 / 190)
+    constexpr int kD = T == 128 ? 1 : 2;
     __shared__ u32x4 left[kD][2][T][4];
     __shared__ __attribute__((aligned(16))) char right[kD][2][MODE == kApply ? kBK * kRow : T * 64];
     const int id = matrix_of(t, blockIdx.x);
@@ -509,7 +516,7 @@ __global__ __launch_bounds__(kBlk) void ns_store_kernel(Table t, char* ws, int t
 
 // ---- small matrices: everything in one workgroup ------------------------------------------------------------------------------------
 // X stays in LDS as binary32 and takes the binary32 matrix instruction (16 x 16 x 4): at 16 x 432 the products are nothing and the 27
-// launches of the general form were 96 us.  Rows lie 4 words apart modulo 64, so 16 rows x 4 words touch every bank once.  The sum over
+// launches of the general form take 105 us, this one 17; 32 x 700 95 and 54, 24 such layers together 110 and 50.  Rows lie 4 words apart modulo 64, so 16 rows x 4 words touch every bank once.  The sum over
 // k runs in any order, so a lane reads four consecutive k at once and gives one to each of four instructions.
 constexpr int kSmallBlk = 1024, kSmallWaves = kSmallBlk / 64, kSmallWords = 32 * 772;
 constexpr int small_width(int rows) { return (kSmallWords / rows - 4) / 64 * 64; }      // 1536 columns of 16 rows, 768 of 32
@@ -636,7 +643,8 @@ bool all_small(const pvx_matrix* mats, int count) {
 
 int round_up(int v, int to) { return PVX_CDIV(v, to) * to; }
 
-// 128 x 128 tiles where the widest product fills the chip with them (they read LDS half as often), 64 x 64 otherwise
+// 128 x 128 tiles where the widest product fills the chip with them (they read LDS half as often), 64 x 64 otherwise (128 / 64:
+// 2048 x 4096 1167 / 1422 us, 2048 x 2048 782 / 884, 1024 x 1024 342 / 257, 512 x 2304 245 / 190)
 int tile_of(const pvx_matrix* mats, int count) {
     double tiles = 0.0;
     for (int i = 0; i < count; i++) tiles += (double)mats[i].rows * mats[i].cols / (128.0 * 128.0);
@@ -644,7 +652,8 @@ int tile_of(const pvx_matrix* mats, int count) {
 }
 
 // Parts of a sum: `slots` workgroups run at a time on 256 CUs; the number of parts that leaves the fewest of them idle in the last turn, of
-// those that fit one turn, a part keeping at least four steps of k
+// those that fit one turn, a part keeping at least four steps of k (with one part: 256 x 2304 280 us instead of 147, 2048 x 4096 1414
+// instead of 1167)
 int parts_of(long long tiles, int k, int tile) {
     const int most = PVX_CDIV(PVX_CDIV(k, kBK), 4), slots = tile == 128 ? 3 : 6;
     int best = 1;
