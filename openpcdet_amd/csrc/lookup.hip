@@ -306,15 +306,16 @@ __global__ __launch_bounds__(kBlk) void lookup_kernel(const E* __restrict__ tabl
     }
 }
 
-// The gradient's sums.  `ch` lanes take a block of kFan positions of the sorted list and walk it, eight rows on their way at a time: they
+// The gradient's sums.  `ch` lanes take a block of 2^fan positions of the sorted list and walk it, eight rows on their way at a time: they
 // add rows up while the key stays, and where it changes the table's row is finished.  A run that crosses a border of the block
 // leaves what the block holds of it: the run that comes in from the left (or is the whole block) as the block's head, the one that goes on
-// to the right as its tail.  Blocks of kFan whole heads, and once more, are added up where they carry one key; then the block in which a
-// crossing run begins joins its tail, whole blocks by the largest that fit, and the last head: at most 2 kWorth + n / kFan^3 steps,
-// whatever share of the list the row has.  (A level is made where the one before has kWorth blocks: 2 us where no run is long, 240 000
-// keys 63 -> 64 us; 1 048 579 skewed keys 337 -> 264.)  All work is in proportion to the list, so the table is cleared beforehand; a
-// walk through each row's run by its offsets instead took 1.7 times as long where the runs' lengths differ much.
-constexpr int kFan = 64, kFanLog = 6, kLevels = 3, kWorth = 256;
+// to the right as its tail.  2^fan heads are added up where they carry one key, and so on by levels; then the block in which a crossing
+// run begins joins its tail, whole blocks by the largest that fit, and the last head: at most 2^fan steps within a block and twice that
+// many blocks on each level, and kWorth of the last, whatever share of the list the row has.  (A level is made where the one before has
+// kWorth blocks: 2 us where no run is long, 240 000 keys 63 -> 64 us; 1 048 579 skewed keys 337 -> 264.)  All work is in proportion to
+// the list, so the table is cleared beforehand; a walk through each row's run by its offsets instead took 1.7 times as long where the
+// runs' lengths differ much.
+constexpr int kLevels = 5, kWorth = 256;
 
 template <typename E, int V> __device__ __forceinline__ void store_row(E* dtable, long long at, const float (&acc)[V], float scale) {
     Pack<E, V> o;
@@ -325,13 +326,13 @@ template <typename E, int V> __device__ __forceinline__ void store_row(E* dtable
 
 template <typename E, int V>
 __global__ __launch_bounds__(kBlk) void run_sum_kernel(const E* __restrict__ dout, const int* __restrict__ order, const int* __restrict__ keys, int n,
-                                                       int m, int ch, int blocks, float scale, float* __restrict__ head, float* __restrict__ tail,
+                                                       int m, int ch, int blocks, int fan, float scale, float* __restrict__ head, float* __restrict__ tail,
                                                        E* __restrict__ dtable) {
     constexpr int U = 8;
     const Lane t(ch);
     for (int k = t.chunk; k < ch; k += kBlk) {
         for (long long blk = t.first(); blk < blocks; blk += t.step()) {
-            const int p0 = (int)blk * kFan, p1 = min(p0 + kFan, n);
+            const int p0 = (int)blk << fan, p1 = min(p0 + (1 << fan), n);
             const int left = p0 > 0 ? keys[p0 - 1] : -1, right = p1 < n ? keys[p1] : -1;
             int key[U + 1], row[U], begin = p0;
             float acc[V];
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(kBlk) void run_sum_kernel(const E* __restrict__ dou
 
 // a level's whole blocks from the level before; shift: log2 of the positions of a block of this level
 __global__ __launch_bounds__(kBlk) void run_next_kernel(const float* __restrict__ in, const int* __restrict__ keys, int m, int width, int blocks,
-                                                        int shift, float* __restrict__ part) {
+                                                        int fan, int shift, float* __restrict__ part) {
     const Lane t(width);
     for (int k = t.chunk; k < width; k += kBlk) {
         for (long long blk = t.first(); blk < blocks; blk += t.step()) {
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(kBlk) void run_next_kernel(const float* __restrict_
             if ((unsigned)key >= (unsigned)m || keys[p0 + (1LL << shift) - 1] != key) continue;
             float acc = 0.f;
 #pragma unroll 16
-            for (int i = 0; i < kFan; i++) acc += in[(blk * kFan + i) * width + k];
+            for (int i = 0; i < 1 << fan; i++) acc += in[((blk << fan) + i) * width + k];
             part[blk * width + k] = acc;
         }
     }
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(kBlk) void run_next_kernel(const float* __restrict_
 
 // first position in (p, end] whose key is not `key`; keys ascend and keys[p] == key
 __device__ __forceinline__ int run_end(const int* keys, int p, int end, int key) {
-    int step = kFan;
+    int step = 32;
     while (p < end - step && keys[p + step] == key) { p += step; step <<= 1; }
     int hi = p < end - step ? p + step : end;
     while (hi - p > 1) { const int mid = p + ((hi - p) >> 1); if (keys[mid] == key) p = mid; else hi = mid; }
@@ -412,28 +413,28 @@ struct Levels { const float *p[kLevels], *tail; int n; };
 
 // the rows of runs that cross a border, each by the block it begins in
 template <typename E, int V>
-__global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ keys, int n, int m, int ch, int blocks, Levels lv, float scale,
+__global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ keys, int n, int m, int ch, int blocks, int fan, Levels lv, float scale,
                                                         E* __restrict__ dtable) {
     const Lane t(ch);
     for (int k = t.chunk; k < ch; k += kBlk) {
         for (long long blk = t.first(); blk < blocks - 1; blk += t.step()) {
-            const int p0 = (int)blk * kFan, v = keys[p0 + kFan - 1];
-            if ((unsigned)v >= (unsigned)m || keys[p0 + kFan] != v) continue;
+            const int p0 = (int)blk << fan, v = keys[p0 + (1 << fan) - 1];
+            if ((unsigned)v >= (unsigned)m || keys[p0 + (1 << fan)] != v) continue;
             const bool whole = keys[p0] == v;
             if (whole && p0 > 0 && keys[p0 - 1] == v) continue;                  // it began further left
             const float* q = (whole ? lv.p[0] : lv.tail) + (blk * ch + k) * V;
             float acc[V];
 #pragma unroll
             for (int j = 0; j < V; j++) acc[j] = q[j];
-            int p = p0 + kFan;
+            int p = p0 + (1 << fan);
             const int end = run_end(keys, p, n, v);
             while (p < end) {
                 int level = 1;                       // the largest aligned block that fits
-                while (level < lv.n && (p & ((kFan << (kFanLog * level)) - 1)) == 0 && p <= end - (kFan << (kFanLog * level))) level++;
+                while (level < lv.n && (p & ((1 << fan * (level + 1)) - 1)) == 0 && p <= end - (1 << fan * (level + 1))) level++;
                 // the blocks of this level up to where a larger one may begin (the last, open one of level 1 is a head), eight at a time
-                const int shift = kFanLog * level, b0 = p >> shift;
-                int b1 = level == 1 ? (int)(((long long)end + kFan - 1) >> kFanLog) : end >> shift;
-                if (level < lv.n) b1 = min(b1, (b0 | (kFan - 1)) + 1);
+                const int shift = fan * level, b0 = p >> shift, last = (int)(((long long)end + (1 << fan) - 1) >> fan);
+                int b1 = level == 1 ? last : end >> shift;
+                if (level < lv.n) b1 = min(b1, (b0 | ((1 << fan) - 1)) + 1);
                 q = lv.p[level - 1] + k * V;
                 for (int b = b0; b < b1; b += 8) {
                     float w[8][V];
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ 
                             for (int j = 0; j < V; j++) acc[j] += w[u][j];
                         }
                 }
-                if (level == 1 && b1 == (int)(((long long)end + kFan - 1) >> kFanLog)) break;
+                if (level == 1 && b1 == last) break;
                 p = b1 << shift;
             }
             store_row<E, V>(dtable, (long long)v * ch + k, acc, scale);
@@ -554,19 +555,29 @@ int vector_of(int width, int dtype, std::initializer_list<const void*> ptrs) {
     return v;
 }
 
-// level 1 has a block for every begun kFan positions, the others for whole ones
-int blocks_of(int n, int level) { return level == 0 ? PVX_CDIV(n, kFan) : n >> (kFanLog * (level + 1)); }
+// log2 of a block's positions: shorter blocks where there are few, so that the chip has work.  Lookup and gradient with blocks chosen / of
+// 64: 5000 x 64 29 / 38 us, 30 000 x 32 37 / 46, 240 000 x 32 58 / 64 (binary32), 100 000 x 64 bf16 50 / 61; with another threshold
+// 500 000 x 64 117 (2^18) and 122 (2^19), 240 000 x 32 58 (2^18) and 63 (2^16); with blocks down to 8, 20 000 x 16 30 / 33.
+int fan_of(int n, int width) {
+    int fan = 6;
+    while (fan > 4 && (long long)(n >> fan) * width < (1 << 18)) fan--;
+    return fan;
+}
+
+// level 1 has a block for every begun 2^fan positions, the others for whole ones
+int blocks_of(int n, int fan, int level) { return level == 0 ? PVX_CDIV(n, 1 << fan) : (int)((long long)n >> (fan * (level + 1))); }
 
 template <typename C> Levels carve_levels(C& cv, int n, int width, float** out, float** tail) {
+    const int fan = fan_of(n, width);
     Levels lv;
     lv.n = 0;
     for (int l = 0; l < kLevels; l++) {
-        const bool worth = l == 0 ? n > kFan : lv.n == l && blocks_of(n, l - 1) >= kWorth;
-        out[l] = worth ? cv.template take<float>((size_t)blocks_of(n, l) * width) : nullptr;
+        const bool worth = l == 0 ? n > 1 << fan : lv.n == l && blocks_of(n, fan, l - 1) >= kWorth;
+        out[l] = worth ? cv.template take<float>((size_t)blocks_of(n, fan, l) * width) : nullptr;
         lv.p[l] = out[l];
         if (worth) lv.n = l + 1;
     }
-    *tail = lv.n > 0 ? cv.template take<float>((size_t)blocks_of(n, 0) * width) : nullptr;
+    *tail = lv.n > 0 ? cv.template take<float>((size_t)blocks_of(n, fan, 0) * width) : nullptr;
     lv.tail = *tail;
     return lv;
 }
@@ -585,17 +596,17 @@ int grad_impl(const E* dout, const int* order, const int* keys, int n, int m, in
     hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(want > 4096 ? 4096 : want)), dim3(kBlk), 0, st, (char*)dtable, bytes);
     PVX_CHECK_LAUNCH();
     if (n == 0) return PVX_OK;
-    const int blocks = blocks_of(n, 0);
-    hipLaunchKernelGGL((run_sum_kernel<E, V>), grid_for(blocks, ch, 1), dim3(kBlk), 0, st, dout, order, keys, n, m, ch, blocks, scale,
+    const int fan = fan_of(n, width), blocks = blocks_of(n, fan, 0);
+    hipLaunchKernelGGL((run_sum_kernel<E, V>), grid_for(blocks, ch, 1), dim3(kBlk), 0, st, dout, order, keys, n, m, ch, blocks, fan, scale,
                        part[0], tail, dtable);
     PVX_CHECK_LAUNCH();
     if (blocks == 1) return PVX_OK;
     for (int l = 1; l < lv.n; l++) {
-        hipLaunchKernelGGL(run_next_kernel, grid_for(blocks_of(n, l), width, 1), dim3(kBlk), 0, st, part[l - 1], keys, m, width, blocks_of(n, l),
-                           kFanLog * (l + 1), part[l]);
+        hipLaunchKernelGGL(run_next_kernel, grid_for(blocks_of(n, fan, l), width, 1), dim3(kBlk), 0, st, part[l - 1], keys, m, width,
+                           blocks_of(n, fan, l), fan, fan * (l + 1), part[l]);
         PVX_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((run_join_kernel<E, V>), grid_for(blocks - 1, ch, 1), dim3(kBlk), 0, st, keys, n, m, ch, blocks, lv, scale, dtable);
+    hipLaunchKernelGGL((run_join_kernel<E, V>), grid_for(blocks - 1, ch, 1), dim3(kBlk), 0, st, keys, n, m, ch, blocks, fan, lv, scale, dtable);
     PVX_CHECK_LAUNCH();
     return PVX_OK;
 }

@@ -1,7 +1,10 @@
 """Rows looked up by index and the table's gradient by sorted index (csrc/lookup.hip; scatter.lookup_rows, scatter.sort_index) against
 plain float64 forms.  The forward is one product rounded once.  A gradient row of k entries is a sum in binary32 along a chain of at
-most 3 * 64 additions inside blocks of three levels and, behind them, a head, a tail, 2 * 255 blocks of two levels and k / 64^3 of the
-third: fewer than 828 + k / 64^3 roundings of partial sums no larger than sum |dout|; then the scale and one rounding more:
+most L F additions inside blocks of L levels (F = 16, 32 or 64 entries; a level is there if the one before has 256 blocks), a tail, 2 (F - 1)
+blocks of each level but the last, and of that one 255 or, on the highest, k / F^L.  F = 16 up to 2^23 entries: L <= 4, 64 + 1 + 90 + 255.
+F = 32 up to 2^24: L <= 4, 128 + 1 + 186 + 255.  F = 64: L = 3, 192 + 1 + 252 + 255, or k / 64^3 for the last; L = 4 (a list of 2^26),
+256 + 1 + 378 + k / 64^4 <= 128.  Fewer than 828 + k / 64^3 roundings of partial sums no
+larger than sum |dout|; then the scale and one rounding more:
 |error| <= (828 + k / 64^3 + 1) * 2^-24 * sum |dout| |scale| + eps / 2 |value|."""
 import pytest
 import torch
