@@ -26,10 +26,28 @@ __device__ __forceinline__ unsigned long long same_digit(int digit, int bits, bo
     return mask;
 }
 
+// Memory to set to zero by `blocks` workgroups.  The gradient's table rides behind the sort's first kernel, which leaves the chip idle,
+// rather than in a launch of its own.
+struct Clear {
+    char* p;
+    long long bytes;
+    int blocks;
+    __device__ __forceinline__ void part(int block, int threads) const {
+        // whole 16-byte pieces between the ends; the allocation begins anywhere
+        const long long head = min(bytes, (long long)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15)), pieces = (bytes - head) / 16;
+        const long long i0 = (long long)block * threads + threadIdx.x, step = (long long)blocks * threads;
+        uint4* q = reinterpret_cast<uint4*>(p + head);
+        for (long long i = i0; i < pieces; i += step) q[i] = make_uint4(0, 0, 0, 0);
+        for (long long i = i0; i < head; i += step) p[i] = 0;
+        for (long long i = head + pieces * 16 + i0; i < bytes; i += step) p[i] = 0;
+    }
+};
+
 // ---- one workgroup sorts everything: up to kOneMax keys, all passes in LDS -----------------------------------------------------
 template <typename I>
 __global__ __launch_bounds__(kOneBlk) void sort_one_kernel(const I* __restrict__ index, int n, int m, int total_bits, int* __restrict__ order,
-                                                           int* __restrict__ keys_out, int* __restrict__ offsets) {
+                                                           int* __restrict__ keys_out, int* __restrict__ offsets, Clear clear) {
+    if (blockIdx.x > 0) { clear.part(blockIdx.x - 1, kOneBlk); return; }
     constexpr int kWaves = kOneBlk / 64, kDigits = 1 << kOneBits;
     __shared__ int skey[kOneMax], sidx[kOneMax];
     __shared__ int cnt[kWaves][kDigits];
@@ -121,8 +139,9 @@ template <> struct From<int2> {
 // hist[tile * by_tile + digit * by_digit]
 template <typename I, int R>
 __global__ __launch_bounds__(kBlk) void sort_count_kernel(const I* __restrict__ in, int n, int m, int shift, int bits, int by_tile, int by_digit,
-                                                          int* __restrict__ hist) {
+                                                          int* __restrict__ hist, int tiles, Clear clear) {
     extern __shared__ int count[];
+    if ((int)blockIdx.x >= tiles) { clear.part(blockIdx.x - tiles, kBlk); return; }
     const int digits = 1 << bits;
     for (int d = threadIdx.x; d < digits; d += kBlk) count[d] = 0;
     __syncthreads();
@@ -457,15 +476,7 @@ __global__ __launch_bounds__(kBlk) void run_join_kernel(const int* __restrict__ 
     }
 }
 
-__global__ __launch_bounds__(kBlk) void clear_kernel(char* __restrict__ p, long long bytes) {
-    // whole 16-byte pieces between the ends; the allocation begins anywhere
-    const long long head = min(bytes, (long long)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15)), pieces = (bytes - head) / 16;
-    const long long i0 = (long long)blockIdx.x * kBlk + threadIdx.x, step = (long long)gridDim.x * kBlk;
-    uint4* q = reinterpret_cast<uint4*>(p + head);
-    for (long long i = i0; i < pieces; i += step) q[i] = make_uint4(0, 0, 0, 0);
-    for (long long i = i0; i < head; i += step) p[i] = 0;
-    for (long long i = head + pieces * 16 + i0; i < bytes; i += step) p[i] = 0;
-}
+__global__ __launch_bounds__(kBlk) void clear_kernel(Clear c) { c.part(blockIdx.x, kBlk); }
 
 int bits_of(int m) {                     // bits of the keys 0 .. m (m >= 1)
     int b = 1;
@@ -493,7 +504,8 @@ template <typename C> void carve_sort(C& cv, int n, SortWs* w) {
 constexpr int kOwnScan = 1 << 14;
 
 template <typename I>
-int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const SortWs& w, int2* out, int* keys, int* order, hipStream_t st) {
+int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const SortWs& w, int2* out, int* keys, int* order, const Clear& clear,
+              hipStream_t st) {
     const int tiles = tiles_of(n), digits = 1 << bits;
     const bool own = (long long)tiles * digits <= kOwnScan;
     const size_t lds = sizeof(int) * ((size_t)digits * (kBlk / 64) + kBlk / 64);
@@ -501,8 +513,8 @@ int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const S
     const int* totals = own ? nullptr : w.totals;
 #define SORT_PASS(R)                                                                                                                             \
     do {                                                                                                                                         \
-        hipLaunchKernelGGL((sort_count_kernel<I, R>), dim3(tiles), dim3(kBlk), sizeof(int) * digits, st, in, n, m, shift, bits, by_tile,         \
-                           by_digit, w.hist);                                                                                                    \
+        hipLaunchKernelGGL((sort_count_kernel<I, R>), dim3(tiles + clear.blocks), dim3(kBlk), sizeof(int) * digits, st, in, n, m, shift, bits,   \
+                           by_tile, by_digit, w.hist, tiles, clear);                                                                             \
         PVX_CHECK_LAUNCH();                                                                                                                      \
         if (!own) {                                                                                                                              \
             hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(64), 0, st, w.hist, tiles, w.totals);                                        \
@@ -522,11 +534,12 @@ int sort_pass(const I* in, int n, int m, int shift, int bits, bool last, const S
 }
 
 template <typename I>
-int sort_impl(const I* index, int n, int m, int* order, int* keys, int* offsets, const SortWs& w, hipStream_t st) {
+int sort_impl(const I* index, int n, int m, int* order, int* keys, int* offsets, const SortWs& w, const Clear& clear, hipStream_t st) {
     const int total_bits = bits_of(m);
     if (n <= kOneMax) {
         const bool inside = offsets && m <= 2 * kOneMax;       // few rows: the same workgroup writes their offsets
-        hipLaunchKernelGGL((sort_one_kernel<I>), dim3(1), dim3(kOneBlk), 0, st, index, n, m, total_bits, order, keys, inside ? offsets : (int*)nullptr);
+        hipLaunchKernelGGL((sort_one_kernel<I>), dim3(1 + clear.blocks), dim3(kOneBlk), 0, st, index, n, m, total_bits, order, keys,
+                           inside ? offsets : (int*)nullptr, clear);
         PVX_CHECK_LAUNCH();
         if (inside) return PVX_OK;
     } else {
@@ -534,8 +547,8 @@ int sort_impl(const I* index, int n, int m, int* order, int* keys, int* offsets,
         for (int p = 0, shift = 0; p < passes; p++) {
             const int bits = PVX_CDIV(total_bits - shift, passes - p);
             int2 *in = p % 2 ? w.even : w.odd, *out = p % 2 ? w.odd : w.even;
-            const int rc = p == 0 ? sort_pass<I>(index, n, m, shift, bits, p == passes - 1, w, out, keys, order, st)
-                                  : sort_pass<int2>(in, n, m, shift, bits, p == passes - 1, w, out, keys, order, st);
+            const int rc = p == 0 ? sort_pass<I>(index, n, m, shift, bits, p == passes - 1, w, out, keys, order, clear, st)
+                                  : sort_pass<int2>(in, n, m, shift, bits, p == passes - 1, w, out, keys, order, Clear{}, st);
             if (rc != PVX_OK) return rc;
             shift += bits;
         }
@@ -582,6 +595,12 @@ template <typename C> Levels carve_levels(C& cv, int n, int width, float** out, 
     return lv;
 }
 
+// workgroups of `threads`, four pieces of 16 bytes a thread and no more than are resident several times
+Clear clear_of(void* p, long long bytes, int threads) {
+    const long long want = PVX_CDIV(bytes, 16LL * threads * 4), most = (1 << 20) / threads;
+    return Clear{(char*)p, bytes, (int)(want > most ? most : want)};
+}
+
 // workgroups for `rows` rows of `ch` chunks, `each` of them a thread
 dim3 grid_for(long long rows, int ch, int each) {
     const long long slots = kBlk / (ch < kBlk ? ch : kBlk), blocks = PVX_CDIV(rows, slots * each);
@@ -592,10 +611,6 @@ template <typename E, int V>
 int grad_impl(const E* dout, const int* order, const int* keys, int n, int m, int width, float scale, E* dtable, float** part, float* tail,
               const Levels& lv, hipStream_t st) {
     const int ch = width / V;
-    const long long bytes = (long long)m * width * sizeof(E), want = PVX_CDIV(bytes, 16LL * kBlk * 4);
-    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(want > 4096 ? 4096 : want)), dim3(kBlk), 0, st, (char*)dtable, bytes);
-    PVX_CHECK_LAUNCH();
-    if (n == 0) return PVX_OK;
     const int fan = fan_of(n, width), blocks = blocks_of(n, fan, 0);
     hipLaunchKernelGGL((run_sum_kernel<E, V>), grid_for(blocks, ch, 1), dim3(kBlk), 0, st, dout, order, keys, n, m, ch, blocks, fan, scale,
                        part[0], tail, dtable);
@@ -675,8 +690,8 @@ extern "C" int pvx_sort_index(const void* index, int index64, int n, int m, int*
     SortWs w;
     carve_sort(cv, n, &w);
     if (!cv.ok()) return PVX_ERR_WORKSPACE;
-    if (index64) return sort_impl<long long>((const long long*)index, n, m, order, keys, offsets, w, st);
-    return sort_impl<int>((const int*)index, n, m, order, keys, offsets, w, st);
+    if (index64) return sort_impl<long long>((const long long*)index, n, m, order, keys, offsets, w, Clear{}, st);
+    return sort_impl<int>((const int*)index, n, m, order, keys, offsets, w, Clear{}, st);
 }
 
 extern "C" int pvx_lookup_rows(const void* table, int dtype, const void* index, int index64, int n, int m, int width, float scale, void* out,
@@ -716,18 +731,23 @@ extern "C" int pvx_lookup_rows_grad(const void* dout, int dtype, const void* ind
     float *part[kLevels], *tail;
     const Levels lv = carve_levels(cv, n, width, part, &tail);
     hipStream_t st = (hipStream_t)stream;
+    const Clear clear = clear_of(dtable, (long long)m * width * (dtype == PVX_F32 ? 4 : 2), !order && n > 0 && n <= kOneMax ? kOneBlk : kBlk);
     if (!order && n > 0) {
         int *own = cv.take<int>(n), *own_keys = cv.take<int>(n);
         SortWs w;
         carve_sort(cv, n, &w);
         if (!cv.ok()) return PVX_ERR_WORKSPACE;
-        const int rc = index64 ? sort_impl<long long>((const long long*)index, n, m, own, own_keys, nullptr, w, st)
-                               : sort_impl<int>((const int*)index, n, m, own, own_keys, nullptr, w, st);
+        const int rc = index64 ? sort_impl<long long>((const long long*)index, n, m, own, own_keys, nullptr, w, clear, st)
+                               : sort_impl<int>((const int*)index, n, m, own, own_keys, nullptr, w, clear, st);
         if (rc != PVX_OK) return rc;
         order = own;
         keys = own_keys;
+    } else {
+        if (!cv.ok()) return PVX_ERR_WORKSPACE;
+        hipLaunchKernelGGL(clear_kernel, dim3(clear.blocks), dim3(kBlk), 0, st, clear);
+        PVX_CHECK_LAUNCH();
+        if (n == 0) return PVX_OK;
     }
-    if (!cv.ok()) return PVX_ERR_WORKSPACE;
     const int v = vector_of(width, dtype, {dout, dtable});
     if (dtype == PVX_F32) return grad_dispatch<float>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
     if (dtype == PVX_F16) return grad_dispatch<_Float16>(dout, order, keys, n, m, width, scale, dtable, part, tail, lv, v, st);
