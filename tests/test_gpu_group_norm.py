@@ -155,6 +155,54 @@ def test_odd_shapes(cuda_device, n, c, groups, cuts):
         check(cuda_device, n, c, groups, cuts=cuts, dtype=dtype, act="silu", eps=1e-3)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,c,groups", [(41000, 96, 8), (41001, 104, 52), (270000, 128, 16), (270001, 128, 32), (34000, 1000, 8)])
+def test_chunks_of_two_and_four_channels(cuda_device, dtype, n, c, groups):
+    """past 2^22 and past 2^25 elements; few enough groups for the applying kernels to finish the statistics, and too many"""
+    check(cuda_device, n, c, groups, cuts=[0, 17, 17, n // 3, n - 100], dtype=dtype, act="silu", res=True, mixed=True)
+
+
+def test_chunks_that_an_address_narrows(cuda_device):
+    check(cuda_device, 270000, 128, 8, cuts=[0, 100000, 270000], dtype=torch.bfloat16, misalign=True)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    rows, c = 2 ** 25 + 4000, 64                              # 2^31 elements end inside the second sample
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    x = torch.randn(rows, c, device=cuda_device, dtype=torch.bfloat16, generator=g).requires_grad_(True)
+    up = torch.randn(rows, c, device=cuda_device, dtype=torch.bfloat16, generator=g)
+    w = (torch.rand(c, device=cuda_device, generator=g) + 0.5).requires_grad_(True)
+    cut = 2 ** 25 - 3000
+    off = torch.tensor([0, cut, rows], dtype=torch.int32, device=cuda_device)
+    y = norm.group_norm_act(x, 8, w, None, act="silu", offsets=off)
+    dx, dw = torch.autograd.grad(y, [x, w], up)
+    for lo, hi, a, b in ((0, 2000, 0, cut), (cut, rows, cut, rows)):      # rows lo .. hi of the sample a .. b
+        mean = torch.zeros(8, dtype=torch.float64, device=cuda_device)
+        square = torch.zeros_like(mean)
+        for k in range(a, b, 2 ** 22):
+            part = x.detach()[k:min(b, k + 2 ** 22)].double().view(-1, 8, 8)
+            mean += part.sum((0, 2))
+            square += part.square().sum((0, 2))
+        count = (b - a) * 8
+        mean, rstd = mean / count, 1 / (square / count - (mean / count).square() + 1e-5).sqrt()
+        rep = lambda v: v.repeat_interleave(8)  # noqa: E731
+        xh = (x.detach()[lo:hi].double() - rep(mean)) * rep(rstd)
+        z = xh * w.detach().double()
+        want = z * torch.sigmoid(z)
+        # z is off by at most 8 roundings of values up to 2 |z| + 1, SiLU's slope is below 1.1, and the result is rounded once: bfloat16 has
+        # steps of 2^-7 in [1, 2), so half a step is at most eps / 2 = 2^-8 of the value
+        half = torch.finfo(torch.bfloat16).eps / 2
+        assert bool(((y.detach()[lo:hi].double() - want).abs() <= half * want.abs() + 16 * U * (2 * z.abs() + 1)).all())
+    # the gradient of the second sample alone, from the same rows in a tensor of their own: the same formula from other pieces
+    tail = x.detach()[cut:].clone().requires_grad_(True)
+    wt = w.detach().clone().requires_grad_(True)
+    dt, = torch.autograd.grad(norm.group_norm_act(tail, 8, wt, None, act="silu", offsets=off[1:] - cut), [tail], up[cut:])
+    # means agree to 2^-23 of the values (at most 3 here), so dx to a few of those before its rounding, where the two may fall to either
+    # side: half a step each, 2 (eps / 2) = 2^-7 of the value
+    assert bool(((dt.double() - dx[cut:].double()).abs() <= 2 * half * dt.double().abs() + 64 * U).all())
+    assert bool(torch.isfinite(dw).all())
+
+
 def test_many_groups_and_samples(cuda_device):
     check(cuda_device, 20000, 2048, 2048, cuts=[0, 20000], act="silu")                   # a group a channel: the widest workgroup's LDS
     check(cuda_device, 20000, 2048, 1, cuts=[0, 9000, 20000], act="silu")

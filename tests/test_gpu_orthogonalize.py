@@ -200,6 +200,27 @@ def test_refusals_on_the_device(cuda_device):
         optim.orthogonalize([m, m.cpu()])
 
 
+def test_offsets_past_32_bits(cuda_device):
+    m, n = 2112, 2 ** 20                                                 # 2.2e9 elements
+    a, b, c = optim.COEFFICIENTS
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x = torch.randn(m, n, device=cuda_device, dtype=torch.bfloat16, generator=g)
+    got = optim.orthogonalize(x, steps=2)
+    gram = torch.zeros(m, m, dtype=torch.float64, device=cuda_device)
+    for k in range(0, n, 2 ** 16):
+        part = x[:, k:k + 2 ** 16].double()
+        gram += part @ part.t().contiguous()
+    norm = float(gram.diagonal().sum().sqrt()) + 1e-7
+    gram /= norm * norm
+    eye = torch.eye(m, dtype=torch.float64, device=cuda_device)
+    total = eye
+    for _ in range(2):                                                   # the products with X come to one matrix: A follows from A
+        step = a * eye + b * gram + c * (gram @ gram)
+        total, gram = step @ total, step @ gram @ step
+    for k in (0, n // 2 - 1000, n - 4096):
+        assert rel(got[:, k:k + 4096], total @ (x[:, k:k + 4096].double() / norm)) <= bound(torch.bfloat16, True, (m, n))
+
+
 def test_muon_refuses_before_it_changes_anything(cuda_device):
     ok, bad = torch.nn.Parameter(torch.ones(4, 4, device=cuda_device)), torch.nn.Parameter(torch.ones(4, 4, device=cuda_device, dtype=torch.float64))
     opt = optim.Muon([ok, bad])
