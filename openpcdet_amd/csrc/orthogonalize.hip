@@ -6,7 +6,7 @@
 //
 // The products run on the f16 matrix cores with each operand split in two: x = hi + lo, hi the rounding of x to 11 bits and lo that of
 // the rest, 22 bits and more together, and three of the four products (lo lo is below 2^-24 of hi hi), accumulated in binary32.
-// Against 64 bits this is as near as binary32 products are (measured: 2.6e-6 and 3.5e-6 for 1001 x 2003), at a third of the f16
+// Against 64 bits this is as near as binary32 products are (1001 x 2003: 1.4e-6, binary32's 3.5e-6), at a third of the f16
 // rate instead of a sixteenth of it, which is what the binary32 instruction has.  f16 has few exponents, so X, A and B are kept times
 // powers of two of each matrix and step: the singular values start below |M| / (|M| + eps), the bound follows them through the
 // polynomial, no entry is larger than the largest singular value, and 2^14 stands for the bound.  hi and lo share a word, so a
@@ -16,8 +16,8 @@
 // B X reads X by rows of k: its fragments come out of LDS transposed (ds_read_b64_tr_b16).  Buffers are padded with zeros to whole
 // tiles, which the products reproduce.
 //
-// Wide matrices are bound by the matrix cores: 2048 x 4096 takes 1167 us for 926 Gflop in f16 (three products each), 794 Tflop/s, where
-// the best library product of bf16 reaches 1054 (8192^3).  Few or narrow ones are bound by their launches, five a step: a backbone's
+// Wide matrices are bound by the matrix cores: 2048 x 4096 takes 1167 to 1236 us (by card) for 926 Gflop in f16 (three products each),
+// 750 to 794 Tflop/s, where the best library product of bf16 reaches 1054 (8192^3); they are busy half of the cycles, LDS 42 %.  Few or narrow ones are bound by their launches, five a step: a backbone's
 // 21 layers take 172 us, of which the products are 23 a step.
 #include "pvx_common.h"
 
