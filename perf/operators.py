@@ -24,37 +24,37 @@ RES8X = ",".join(["16x135"] + ["16x432"] * 4 + ["32x432"] + ["32x864"] * 4 + ["6
 def listed():
     return [
         # one frame's deepest level in serving: the launch is what counts
-        dict(name="norm few rows", op="norm", rows=300, samples=1, channels=16, groups=4, dtype="float32", act="relu", residual=False,
+        dict(name="norm, few rows", op="norm", rows=300, samples=1, channels=16, groups=4, dtype="float32", act="relu", residual=False,
              layout="ragged", train=False),
         # the second normalisation of a residual block at a middle level, four frames, forward and backward
-        dict(name="norm residual block step", op="norm", rows=117301, samples=4, channels=64, groups=8, dtype="bfloat16", act="silu",
+        dict(name="norm, residual block step", op="norm", rows=117301, samples=4, channels=64, groups=8, dtype="bfloat16", act="silu",
              residual=True, layout="ragged", train=True),
         # a dense bird's-eye map kept channels last, 188 x 188 cells of three frames, groups of 3 channels
-        dict(name="norm dense map", op="norm", rows=3 * 188 * 188, samples=3, channels=96, groups=32, dtype="float16", act="relu",
+        dict(name="norm, dense map", op="norm", rows=3 * 188 * 188, samples=3, channels=96, groups=32, dtype="float16", act="relu",
              residual=False, layout="dense", train=False),
         # the widest level of a large training batch, forward and backward in 32 bits
-        dict(name="norm widest level step", op="norm", rows=520013, samples=8, channels=128, groups=16, dtype="float32", act="gelu",
+        dict(name="norm, widest level step", op="norm", rows=520013, samples=8, channels=128, groups=16, dtype="float32", act="gelu",
              residual=False, layout="ragged", train=True),
         # class rows for the boxes that one head keeps in serving
-        dict(name="lookup kept boxes", op="lookup", tokens=83, rows=10, width=64, dtype="float32", index="int64", spread="uniform",
+        dict(name="lookup, kept boxes", op="lookup", tokens=83, rows=10, width=64, dtype="float32", index="int64", spread="uniform",
              outside=0.0, scale=8.0, train=False),
         # points of a frame look their voxel's features up (a dynamic encoder's second layer); 5 % lie outside the range
-        dict(name="lookup points in voxels", op="lookup", tokens=240000, rows=31007, width=32, dtype="float32", index="int32",
+        dict(name="lookup, points in voxels", op="lookup", tokens=240000, rows=31007, width=32, dtype="float32", index="int32",
              spread="scan", outside=0.05, scale=1.0, train=True),
         # a table much longer than the list, rows of odd width
-        dict(name="lookup sparse in long table", op="lookup", tokens=70001, rows=999983, width=37, dtype="float16", index="int64",
+        dict(name="lookup, sparse in long table", op="lookup", tokens=70001, rows=999983, width=37, dtype="float16", index="int64",
              spread="uniform", outside=0.0, scale=6.0, train=True),
         # a large table under a skewed distribution: one row takes a large share of the list
-        dict(name="lookup large and skewed", op="lookup", tokens=1048579, rows=250007, width=128, dtype="bfloat16", index="int64",
+        dict(name="lookup, large and skewed", op="lookup", tokens=1048579, rows=250007, width=128, dtype="bfloat16", index="int64",
              spread="skewed", outside=0.0, scale=math.sqrt(128.0), train=True),
         # one narrow layer: latency
-        dict(name="orthogonalize one layer", op="orthogonalize", shapes="16x432", dtype="float32"),
+        dict(name="orthogonalize, one layer", op="orthogonalize", shapes="16x432", dtype="float32"),
         # every convolution of a residual backbone, as an optimiser's step has them
-        dict(name="orthogonalize backbone", op="orthogonalize", shapes=RES8X, dtype="float32"),
+        dict(name="orthogonalize, backbone", op="orthogonalize", shapes=RES8X, dtype="float32"),
         # odd sizes, one taller than wide
-        dict(name="orthogonalize odd layers", op="orthogonalize", shapes="1001x2003,1201x577,77x333", dtype="float32"),
+        dict(name="orthogonalize, odd layers", op="orthogonalize", shapes="1001x2003,1201x577,77x333", dtype="float32"),
         # one wide dense layer
-        dict(name="orthogonalize wide layer", op="orthogonalize", shapes="2048x4096", dtype="bfloat16"),
+        dict(name="orthogonalize, wide layer", op="orthogonalize", shapes="2048x4096", dtype="bfloat16"),
     ]
 
 
