@@ -224,5 +224,11 @@ def raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def check_counts(what, *counts):
+    """the C entries take counts as int, and ctypes drops what is above 32 bits without a word"""
+    if max(counts) > 0x7fffffff:
+        raise ValueError("%s: a count of %s is past 32 bits" % (what, max(counts)))
+
+
 def workspace(nbytes, device):
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)

@@ -107,6 +107,7 @@ def sort_index(index, num_rows):
     num_rows = int(num_rows)
     if num_rows < 1:
         raise ValueError("num_rows must be at least 1, got %d" % num_rows)
+    _lib.check_counts("sort_index", num_rows, index.numel())
     index = index.reshape(-1).contiguous()
     n, dev = index.shape[0], index.device
     L = _lib.lib()
@@ -191,6 +192,7 @@ def lookup_rows(table, index, scale=1.0, sort=None):
     width = 1
     for d in table.shape[1:]:
         width *= d
+    _lib.check_counts("lookup_rows", table.shape[0], width, index.numel())
     flat = table.contiguous() if table.dim() == 2 else table.reshape(table.shape[0], width).contiguous()
     idx = index.contiguous() if index.dim() == 1 else index.reshape(-1).contiguous()
     if torch.is_grad_enabled() and flat.requires_grad:

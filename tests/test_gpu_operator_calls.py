@@ -1,0 +1,27 @@
+"""Calls of the training-step operators (csrc/group_norm.hip, csrc/lookup.hip, csrc/orthogonalize.hip and their Python entries) that the
+tests by operator leave out: other derivatives, sizes past 32 bits, special values, hooks, caches, optimiser options and states."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from openpcdet_amd import backbones, optim, scatter, vfe
+from openpcdet_amd.spconv import pytorch as spconv
+from openpcdet_amd.spconv.pytorch import norm
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+# ---- sizes past 32 bits ----------------------------------------------------------------------------------------------------
+def test_lookup_refuses_counts_past_32_bits(cuda_device):
+    """2^32 + 5 is 5 in 32 bits.  The tensors are expanded from one element: refused before anything of that size is made"""
+    big = 2 ** 32 + 5
+    one, zero = torch.zeros(1, 1, dtype=torch.bfloat16, device=cuda_device), torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    for call in (lambda: scatter.lookup_rows(one.expand(big, 1), zero), lambda: scatter.lookup_rows(one, zero.expand(big)),
+                 lambda: scatter.lookup_rows(one.expand(2, big), zero), lambda: scatter.sort_index(zero, big),
+                 lambda: scatter.sort_index(zero.expand(big), 4)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
