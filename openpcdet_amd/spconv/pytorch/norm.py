@@ -308,6 +308,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, re
         samples = offsets.shape[0] - 1
         if samples < 1:
             raise ValueError("offsets must have an entry more than there are samples")
+    _lib.check_counts("group_norm_act", x.numel() // c, c, samples)
+    if offsets is not None:
         offsets = offsets.contiguous()
         order = order.contiguous() if order is not None else None
     plain = x.dim() == 2

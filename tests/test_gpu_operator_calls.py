@@ -25,3 +25,13 @@ def test_lookup_refuses_counts_past_32_bits(cuda_device):
                  lambda: scatter.sort_index(zero.expand(big), 4)):
         with pytest.raises(ValueError, match="32 bits"):
             call()
+
+
+def test_group_norm_refuses_counts_past_32_bits(cuda_device):
+    big = 2 ** 32 + 5
+    one, off = torch.zeros(1, 1, dtype=torch.bfloat16, device=cuda_device), torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    for call in (lambda: norm.group_norm_act(one.expand(big, 1), 1, offsets=off), lambda: norm.group_norm_act(one.expand(big, 1), 1),
+                 lambda: norm.group_norm_act(one.expand(1, big), 1), lambda: norm.group_norm_act(one.unsqueeze(0).expand(1, big, 1), 1),
+                 lambda: norm.group_norm_act(one, 1, offsets=off[:1].expand(big))):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
