@@ -7,6 +7,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PVX_LIB") or os.path.join(_HERE, "lib", "libpcdet_mi355.so")   # PVX_LIB: a diagnostic build of the same library
@@ -222,6 +223,12 @@ def on(device):
 def raw_stream(device):
     """the current stream of `device` as ctypes takes it"""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def differentiated(*tensors):
+    """whether a call has to go through its autograd function: a gradient is wanted, or some tensor may carry a tangent (which
+    requires_grad does not tell, and which the function refuses)"""
+    return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def check_counts(what, *counts):

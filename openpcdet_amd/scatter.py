@@ -195,7 +195,7 @@ def lookup_rows(table, index, scale=1.0, sort=None):
     _lib.check_counts("lookup_rows", table.shape[0], width, index.numel())
     flat = table.contiguous() if table.dim() == 2 else table.reshape(table.shape[0], width).contiguous()
     idx = index.contiguous() if index.dim() == 1 else index.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and flat.requires_grad:
+    if _lib.differentiated(flat):
         out = _LookupRows.apply(flat, idx, float(scale), sort)
     else:
         out = _lookup(flat, idx, float(scale))

@@ -322,7 +322,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, re
     w = weight.contiguous() if weight is not None else None
     b = bias.contiguous() if bias is not None else None
     args = (flat, w, b, res, offsets, order, samples, num_groups, eps, _ACTS[act])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if _lib.differentiated(*args[:4]):
         y = _GroupNormAct.apply(*args)
     else:
         y = _group_norm_fwd(*args)[0]

@@ -35,3 +35,27 @@ def test_group_norm_refuses_counts_past_32_bits(cuda_device):
                  lambda: norm.group_norm_act(one, 1, offsets=off[:1].expand(big))):
         with pytest.raises(ValueError, match="32 bits"):
             call()
+
+
+# ---- forward-mode derivatives ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(cuda_device, grad):
+    """no forward-mode derivative is defined: refused, not taken for zero"""
+    x, w, r = (torch.randn(s, device=cuda_device) for s in ((6, 8), (8,), (6, 8)))
+    index = torch.tensor([0, 5, 2], device=cuda_device)
+    plain = norm.group_norm_act(x, 2, w, act="relu", residual=r), scatter.lookup_rows(x, index)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: norm.group_norm_act(dual(x), 2, w), lambda: norm.group_norm_act(x, 2, dual(w)),
+                     lambda: norm.group_norm_act(x, 2, w, dual(w)), lambda: norm.group_norm_act(x, 2, residual=dual(r)),
+                     lambda: scatter.lookup_rows(dual(x), index)):
+            with pytest.raises(RuntimeError):
+                call()
+        assert torch.equal(norm.group_norm_act(x, 2, w, act="relu", residual=r), plain[0])      # nothing dual: as ever
+        assert torch.equal(scatter.lookup_rows(x, index), plain[1])
+    with torch.set_grad_enabled(grad):
+        for f in (lambda t: norm.group_norm_act(t, 2, w), lambda t: scatter.lookup_rows(t, index)):
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(f, (x,), (torch.ones_like(x),))
+            with pytest.raises(RuntimeError):
+                torch.func.vmap(f)(x.expand(3, 6, 8))
