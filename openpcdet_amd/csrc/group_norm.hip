@@ -108,7 +108,7 @@ struct Rows {
         }
         int lo = 0, hi = samples;
         while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
+            const int mid = lo + ((hi - lo) >> 1);           // lo + hi passes 2^31 from 2^30 samples on
             if (begin(mid + 1) > p) hi = mid; else lo = mid + 1;
         }
         return lo;

@@ -59,3 +59,15 @@ def test_forward_mode_is_refused(cuda_device, grad):
                 torch.func.jvp(f, (x,), (torch.ones_like(x),))
             with pytest.raises(RuntimeError):
                 torch.func.vmap(f)(x.expand(3, 6, 8))
+
+
+# ---- the largest sizes of the norm -----------------------------------------------------------------------------------------
+def test_norm_of_more_than_2_30_samples(cuda_device):
+    """the rows are those of the last sample: the search for it adds up sample numbers past 2^31"""
+    samples, n = 2 ** 30 + 1000, 700
+    off = torch.zeros(samples + 1, dtype=torch.int32, device=cuda_device)
+    off[-1] = n
+    x = torch.randn(n, 1, device=cuda_device)
+    y = norm.group_norm_act(x, 1, offsets=off)
+    want = norm.group_norm_act(x, 1, offsets=torch.tensor([0, n], dtype=torch.int32, device=cuda_device))
+    assert float((y - want).abs().max()) <= 8 * U * float(want.abs().max() + 1)
