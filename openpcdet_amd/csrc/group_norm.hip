@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_sums_kernel(const E* __res
     __shared__ double red[2 * kBlk * (V + 1)];
     extern __shared__ double per_group[];                // [groups][2]
     const Place t = place<V>(c);
-    const int p0 = blockIdx.x * range, p1 = min(rows.n, p0 + range);
+    const int p0 = blockIdx.x * range, p1 = p0 + min(rows.n - p0, range);
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), lo = max(p0, begin), hi = min(p1, rows.begin(s + 1));
         if (begin >= p1) break;
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_apply_kernel(const E* __re
                                                          float* __restrict__ rstd, E* __restrict__ y) {
     extern __shared__ double per_group[];
     const Place t = place<V>(c);
-    const int p0 = blockIdx.x * range, p1 = min(rows.n, p0 + range), cpg = c / groups;
+    const int p0 = blockIdx.x * range, p1 = p0 + min(rows.n - p0, range), cpg = c / groups;
     const float zero[V] = {};
     float w[V], b[V];
 #pragma unroll
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_sums_kernel(const E* _
     __shared__ double red[2 * kBlk * (V + 1)];
     extern __shared__ double per_group[];
     const Place t = place<V>(c);
-    const int p0 = blockIdx.x * range, p1 = min(rows.n, p0 + range), cpg = c / groups;
+    const int p0 = blockIdx.x * range, p1 = p0 + min(rows.n - p0, range), cpg = c / groups;
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), lo = max(p0, begin), hi = min(p1, rows.begin(s + 1));
         if (begin >= p1) break;
@@ -483,7 +483,7 @@ __device__ __forceinline__ void channel_finish(const double* partial, const Rows
                                                double* red) {
     double a = 0.0, b = 0.0;
     // as many lanes a sample as it has pieces on average, so that the samples are not walked one after the other
-    const int average = PVX_CDIV(PVX_CDIV(rows.n, range), rows.samples) + 1;
+    const int average = (rows.n - 1) / range / rows.samples + 2;
     int lanes = 1;
     while (lanes < average && lanes < kBlk) lanes <<= 1;
     for (int s = threadIdx.x / lanes; s < rows.samples; s += kBlk / lanes) {
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_apply_kernel(const E* 
         return;
     }
     const Place t = place<V>(c);
-    const int p0 = blockIdx.x * range, p1 = min(rows.n, p0 + range), cpg = c / groups;
+    const int p0 = blockIdx.x * range, p1 = p0 + min(rows.n - p0, range), cpg = c / groups;
     const float zero[V] = {};
     int done = p0;
     for (int s = rows.first(p0); s < rows.samples; s++) {
@@ -846,7 +846,7 @@ Shape shape_of(int n, int c, int groups, int v) {
     s.tiles = PVX_CDIV(ch, s.tw);
     const long long r = PVX_CDIV((long long)n, (long long)kTargetBlocks);
     s.range = (int)(PVX_CDIV(r < 2LL * s.rpb ? 2LL * s.rpb : r, (long long)s.rpb) * s.rpb);
-    s.blocks = PVX_CDIV(n, s.range);
+    s.blocks = (int)PVX_CDIV((long long)n, (long long)s.range);      // n + range may pass 2^31
     s.merged = s.tiles == 1 && (long long)s.blocks * groups <= kMergedSums;
     return s;
 }

@@ -71,3 +71,35 @@ def test_norm_of_more_than_2_30_samples(cuda_device):
     y = norm.group_norm_act(x, 1, offsets=off)
     want = norm.group_norm_act(x, 1, offsets=torch.tensor([0, n], dtype=torch.int32, device=cuda_device))
     assert float((y - want).abs().max()) <= 8 * U * float(want.abs().max() + 1)
+
+
+def test_norm_of_nearly_2_31_rows(cuda_device):
+    """one channel, rows up to the largest count that is taken: the last workgroup's range ends past 2^31"""
+    n = 2 ** 31 - 2 ** 20 - 1
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    x = torch.empty(n, 1, dtype=torch.float16, device=cuda_device)
+    x.normal_(generator=g)
+    cut = n - 5000000                                          # the last sample lies in the last two ranges
+    off = torch.tensor([0, cut, n], dtype=torch.int32, device=cuda_device)
+    up = torch.empty_like(x)
+    up.normal_(generator=g)
+    y = norm.group_norm_act(x.requires_grad_(True), 1, offsets=off)
+    dx, = torch.autograd.grad(y, x, up)
+    x, y = x.detach(), y.detach()
+    for lo, hi, a, b in ((0, 1000, 0, cut), (cut - 1000, cut, 0, cut), (cut, n, cut, n)):
+        mean = square = 0.0
+        for k in range(a, b, 2 ** 28):
+            part = x[k:min(b, k + 2 ** 28)].double()
+            mean, square = mean + float(part.sum()), square + float(part.square().sum())
+        mean, square = mean / (b - a), square / (b - a)
+        want = (x[lo:hi].double() - mean) / (square - mean * mean + 1e-5) ** 0.5
+        # five roundings of 32 bits and one of 16
+        tol = 8 * U * (want.abs() + 1) + 2.0 ** -25
+        assert bool(((y[lo:hi].double() - want).abs() <= tol + 2.0 ** -11 * (want.abs() + tol)).all())
+    # of the last sample, whole: xhat is `want`, and dx = (dy - mean dy - xhat mean(dy xhat)) / sqrt(var + eps), a dozen roundings of terms
+    # no larger than |dy| + |mean| + |xhat mean|
+    d = up[cut:].double()
+    m0, m1 = d.mean(), (d * want).mean()
+    terms = (d.abs() + m0.abs() + (want * m1).abs() + 1) / (square - mean * mean + 1e-5) ** 0.5
+    slope = (d - m0 - want * m1) / (square - mean * mean + 1e-5) ** 0.5
+    assert bool(((dx[cut:].double() - slope).abs() <= 16 * U * terms + 2.0 ** -25 + 2.0 ** -11 * slope.abs() * (1 + 2.0 ** -10)).all())
