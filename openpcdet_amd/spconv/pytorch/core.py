@@ -213,17 +213,18 @@ class SparseConvTensor:
 
     def _sample_rows(self):
         """(offsets [batch_size + 1], order [N], both int32): sample b has the rows order[offsets[b]:offsets[b + 1]], in ascending order;
-        rows whose batch index is outside the batch come last.  Kept like the site index, for calls on the same stream (another one has not
-        waited for the sort); listed anew in a graph capture, whose replays may find other indices and whose memory is the graph's."""
+        rows whose batch index is outside the batch come last.  Kept like the site index, for the same batch_size and calls on the same
+        stream (another one has not waited for the sort); listed anew in a graph capture, whose replays may find other indices and whose
+        memory is the graph's."""
         from ...scatter import sort_index
         if torch.cuda.is_current_stream_capturing():
             s = sort_index(self.indices[:, 0], self.batch_size)
             return s.offsets, s.order
-        c, stream = self._sample_holder[0], _lib.raw_stream(self.indices.device)
-        if c is not None and c[0].valid_for(self.indices) and c[3] == stream:
+        c, kept_for = self._sample_holder[0], (self.batch_size, _lib.raw_stream(self.indices.device))
+        if c is not None and c[0].valid_for(self.indices) and c[3] == kept_for:
             return c[1], c[2]
         s = sort_index(self.indices[:, 0], self.batch_size)
-        self._sample_holder[0] = (_SiteIndexCache(self.indices, None, None, None), s.offsets, s.order, stream)
+        self._sample_holder[0] = (_SiteIndexCache(self.indices, None, None, None), s.offsets, s.order, kept_for)
         return s.offsets, s.order
 
     # ---- dense() --------------------------------------------------------------------------------------

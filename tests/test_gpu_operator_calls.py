@@ -103,3 +103,22 @@ def test_norm_of_nearly_2_31_rows(cuda_device):
     terms = (d.abs() + m0.abs() + (want * m1).abs() + 1) / (square - mean * mean + 1e-5) ** 0.5
     slope = (d - m0 - want * m1) / (square - mean * mean + 1e-5) ** 0.5
     assert bool(((dx[cut:].double() - slope).abs() <= 16 * U * terms + 2.0 ** -25 + 2.0 ** -11 * slope.abs() * (1 + 2.0 ** -10)).all())
+
+
+# ---- hooks and subclasses --------------------------------------------------------------------------------------------------
+def _sites(dev, c, batch=3, seed=1):
+    r = np.random.default_rng(seed)
+    coords = np.unique(np.stack([r.integers(0, batch, 2500), r.integers(0, 8, 2500), r.integers(0, 20, 2500), r.integers(0, 20, 2500)], 1), axis=0)
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return torch.randn(len(coords), c, device=dev, generator=g), torch.from_numpy(coords.astype(np.int32)).to(dev)
+
+
+# ---- the list of each frame's rows -----------------------------------------------------------------------------------------
+def test_sample_rows_follow_the_batch_size(cuda_device):
+    feats, idx = _sites(cuda_device, 16)
+    gn = spconv.SparseGroupNorm(4, 16).to(cuda_device)
+    want = gn(spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)).features
+    x = spconv.SparseConvTensor(feats, idx, [8, 20, 20], 2)
+    assert float(gn(x).features[idx[:, 0] == 2].abs().max()) == 0      # rows of no frame
+    x.batch_size = 3
+    assert torch.equal(gn(x).features, want)
