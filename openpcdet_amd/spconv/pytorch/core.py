@@ -215,12 +215,13 @@ class SparseConvTensor:
         """(offsets [batch_size + 1], order [N], both int32): sample b has the rows order[offsets[b]:offsets[b + 1]], in ascending order;
         rows whose batch index is outside the batch come last.  Kept like the site index, for the same batch_size and calls on the same
         stream (another one has not waited for the sort); listed anew in a graph capture, whose replays may find other indices and whose
-        memory is the graph's."""
+        memory is the graph's; what was listed in inference mode is for calls in it (no other can save it for a backward), and indices made
+        there have no version to tell whether they were written to."""
         from ...scatter import sort_index
-        if torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing() or self.indices.is_inference():
             s = sort_index(self.indices[:, 0], self.batch_size)
             return s.offsets, s.order
-        c, kept_for = self._sample_holder[0], (self.batch_size, _lib.raw_stream(self.indices.device))
+        c, kept_for = self._sample_holder[0], (self.batch_size, _lib.raw_stream(self.indices.device), torch.is_inference_mode_enabled())
         if c is not None and c[0].valid_for(self.indices) and c[3] == kept_for:
             return c[1], c[2]
         s = sort_index(self.indices[:, 0], self.batch_size)

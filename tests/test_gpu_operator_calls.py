@@ -122,3 +122,19 @@ def test_sample_rows_follow_the_batch_size(cuda_device):
     assert float(gn(x).features[idx[:, 0] == 2].abs().max()) == 0      # rows of no frame
     x.batch_size = 3
     assert torch.equal(gn(x).features, want)
+
+
+def test_sample_rows_of_inference_mode(cuda_device):
+    feats, idx = _sites(cuda_device, 16)
+    gn = spconv.SparseGroupNorm(4, 16).to(cuda_device)
+    want = gn(spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)).features.detach()
+    x = spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)
+    with torch.inference_mode():
+        assert torch.equal(gn(x).features, want)
+        inside = spconv.SparseConvTensor(feats.clone(), idx.clone(), [8, 20, 20], 3)      # tensors of inference mode: no version counter
+        assert torch.equal(gn(inside).features, want)
+    f = feats.clone().requires_grad_(True)
+    y = gn(x.replace_feature(f)).features                      # a training call on the same sites
+    assert torch.equal(y.detach(), want)
+    y.square().sum().backward()
+    assert f.grad is not None and gn.weight.grad is not None
