@@ -80,7 +80,7 @@ __device__ __forceinline__ float act_of(float z, int act) {
 }
 
 __device__ __forceinline__ float slope_of(float z, int act) {
-    if (act == PVX_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == PVX_ACT_RELU) return z <= 0.f ? 0.f : 1.f;     // a NaN lets the gradient through
     if (act == PVX_ACT_SILU) {
         const float p = sigmoid(z);
         return p * (1.f + z * (1.f - p));

@@ -138,3 +138,24 @@ def test_sample_rows_of_inference_mode(cuda_device):
     assert torch.equal(y.detach(), want)
     y.square().sum().backward()
     assert f.grad is not None and gn.weight.grad is not None
+
+
+# ---- special values --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [200, 20000])
+def test_relu_passes_the_gradient_of_nan(cuda_device, n, dtype):
+    """relu's slope is 0 only where z <= 0: a NaN keeps the gradient that came in, so a loss that has gone wrong shows"""
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    x = torch.randn(n, 16, device=cuda_device, generator=g).to(dtype)
+    x[3, 5] = float("nan")
+    res = torch.randn(n, 16, device=cuda_device, generator=g).to(dtype).requires_grad_(True)
+    b = torch.randn(16, device=cuda_device, generator=g).requires_grad_(True)
+    up = torch.randn(n, 16, device=cuda_device, generator=g).to(dtype)
+    off = torch.tensor([0, n // 2, n], dtype=torch.int32, device=cuda_device)
+    y = norm.group_norm_act(x, 4, None, b, act="relu", residual=res, offsets=off)
+    dres, db = torch.autograd.grad(y, [res, b], up)
+    # torch's own rule on the same outputs
+    assert torch.equal(dres, torch.where(y <= 0, torch.zeros_like(up), up))
+    assert bool(torch.isnan(y[:n // 2, 4:8]).all())
+    want = torch.where(y <= 0, torch.zeros_like(up), up).double().sum(0)
+    assert bool(((db.double() - want).abs() <= U * want.abs() + 1e-30).all())        # sums in 64 bits, rounded once
