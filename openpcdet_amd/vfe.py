@@ -120,6 +120,8 @@ class DynamicMeanVFE(_VFEBase):
 
 
 class PFNLayerV2(nn.Module):
+    inside = False      # unq_inv holds no negative entries (they count from the end, as in any indexing): said by encoders that drop them
+
     def __init__(self, in_channels, out_channels, use_norm=True, last_layer=False):
         super().__init__()
         self.last_vfe = last_layer
@@ -142,7 +144,8 @@ class PFNLayerV2(nn.Module):
             return x_max
         if x_max.dtype not in _lib.DTYPE_CODE or unq_inv.dtype not in (torch.int32, torch.int64):
             return torch.cat([x, x_max[unq_inv.long(), :]], dim=1)
-        return torch.cat([x, lookup_rows(x_max, unq_inv)], dim=1)
+        at = unq_inv if self.inside else torch.where(unq_inv < 0, unq_inv + x_max.shape[0], unq_inv)
+        return torch.cat([x, lookup_rows(x_max, at)], dim=1)
 
 
 class _DynamicPFNVFE(_VFEBase):
@@ -164,6 +167,8 @@ class _DynamicPFNVFE(_VFEBase):
         nf = [num_point_features] + self.num_filters
         self.pfn_layers = nn.ModuleList([PFNLayerV2(nf[i], nf[i + 1], self.use_norm, last_layer=(i >= len(nf) - 2))
                                          for i in range(len(nf) - 1)])
+        for layer in self.pfn_layers:
+            layer.inside = True
         self.voxel_size, self.grid_size, self.point_cloud_range = list(voxel_size), list(grid_size), list(point_cloud_range)
 
     def _extra_features(self):

@@ -159,3 +159,42 @@ def test_relu_passes_the_gradient_of_nan(cuda_device, n, dtype):
     assert bool(torch.isnan(y[:n // 2, 4:8]).all())
     want = torch.where(y <= 0, torch.zeros_like(up), up).double().sum(0)
     assert bool(((db.double() - want).abs() <= U * want.abs() + 1e-30).all())        # sums in 64 bits, rounded once
+
+
+# ---- second derivatives and indices from the end through the voxel encoders ------------------------------------------------
+def _encoder_layer(dev):
+    """a PFNLayerV2, its input, indices that count from the end among them, and what x_max[unq_inv] makes of it"""
+    torch.manual_seed(3)
+    layer = vfe.PFNLayerV2(10, 32, use_norm=False).to(dev)
+    inv = torch.randint(-500, 500, (4000,), device=dev, dtype=torch.int32)
+
+    def plain(a):
+        h = layer.relu(layer.linear(a))
+        return torch.cat([h, scatter.scatter_max(h, inv, dim=0, dim_size=500)[0][inv.long(), :]], dim=1)
+
+    return layer, torch.randn(4000, 10, device=dev), inv, plain
+
+
+def test_voxel_encoder_layer_counts_from_the_end(cuda_device):
+    layer, x, inv, plain = _encoder_layer(cuda_device)
+    results = []
+    for f in (lambda a: layer(a, inv, 500), lambda a: layer(a, inv.long(), 500), plain):
+        a = x.clone().requires_grad_(True)
+        out = f(a)
+        results.append((out.detach(), torch.autograd.grad((out ** 2).sum(), a)[0]))
+    for got in results[:2]:
+        assert torch.equal(got[0], results[2][0])
+        assert float((got[1] - results[2][1]).norm()) <= 1e-5 * float(results[2][1].norm())      # sums of some 20 terms, in another order
+
+
+def test_voxel_encoders_take_the_lookup(cuda_device, monkeypatch):
+    calls = []
+    real = vfe.lookup_rows
+    monkeypatch.setattr(vfe, "lookup_rows", lambda t, i, **kw: calls.append(int(i.min())) or real(t, i, **kw))
+    enc = vfe.DynamicVoxelVFE(dict(USE_NORM=True, WITH_DISTANCE=False, USE_ABSLOTE_XYZ=True, NUM_FILTERS=[32, 16]), 4, [0.25, 0.25, 0.1], [64, 64, 40],
+                              [0.0, -8.0, -2.0, 16.0, 8.0, 2.0]).to(cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    pts = torch.rand(3000, 5, device=cuda_device, generator=g) * torch.tensor([0.0, 20.0, 16.0, 4.0, 1.0], device=cuda_device) \
+        - torch.tensor([0.0, 0.0, 8.0, 2.0, 0.0], device=cuda_device)
+    enc({"points": pts, "batch_size": 1})                                  # a fifth of the points lies outside
+    assert len(calls) == 1 and calls[0] >= 0
