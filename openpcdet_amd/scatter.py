@@ -7,7 +7,6 @@ pvx_scatter_mean / pvx_scatter_max; both are differentiable (PFN weights train t
 `lookup_rows` is the way back, rows of a table picked by index (times a scale), with the table's gradient summed by sorted index
 (pvx_lookup_rows, pvx_sort_index, pvx_lookup_rows_grad); `sort_index` hands that sort out, for an index that several calls share."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -141,18 +140,37 @@ class _LookupRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, sort):
         ctx.save_for_backward(index)
-        ctx.scale, ctx.sort, ctx.shape = scale, sort, table.shape
+        ctx.scale, ctx.sort, ctx.rows = scale, sort, table.shape[0]
         return _lookup(table, index, scale)
 
     @staticmethod
     def backward(ctx, grad):
-        return _lookup_grad_once(ctx, grad) if torch.is_grad_enabled() else _lookup_grad(ctx, grad)
+        index, = ctx.saved_tensors
+        f = _LookupRowsGrad.apply if torch.is_grad_enabled() else _lookup_grad
+        return f(grad, index, ctx.scale, ctx.sort, ctx.rows), None, None, None
 
 
-def _lookup_grad(ctx, grad):
-    index, = ctx.saved_tensors
-    m, w = ctx.shape
-    n, dev, sort = index.shape[0], index.device, ctx.sort
+class _LookupRowsGrad(torch.autograd.Function):
+    """the gradient, under create_graph: linear as the lookup is, and its own gradient is the lookup"""
+
+    @staticmethod
+    def forward(ctx, grad, index, scale, sort, m):
+        ctx.save_for_backward(index)
+        ctx.scale, ctx.sort = scale, sort
+        return _lookup_grad(grad, index, scale, sort, m)
+
+    @staticmethod
+    def backward(ctx, dtable):
+        index, = ctx.saved_tensors
+        dtable = dtable.contiguous()
+        out = _LookupRows.apply(dtable, index, ctx.scale, ctx.sort) if torch.is_grad_enabled() else _lookup(dtable, index, ctx.scale)
+        return out, None, None, None, None
+
+
+def _lookup_grad(grad, index, scale, sort, m):
+    """grad [n, w], index [n] contiguous -> [m, w]"""
+    n, w = grad.shape
+    dev = index.device
     grad = grad.contiguous()
     dtable = grad.new_empty((m, w))
     if m > 0 and w > 0:
@@ -162,20 +180,17 @@ def _lookup_grad(ctx, grad):
             ws = grad.new_empty(size, dtype=torch.uint8)
             order, keys = (sort.order.data_ptr(), sort.keys.data_ptr()) if sort is not None else (None, None)
             rc = L.pvx_lookup_rows_grad(grad.data_ptr(), _lib.DTYPE_CODE[grad.dtype], index.data_ptr(), index.dtype == torch.int64, order, keys,
-                                        n, m, w, ctx.scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
+                                        n, m, w, scale, dtable.data_ptr(), ws.data_ptr(), size, _lib.raw_stream(dev))
             if rc:
                 _lib.check(rc, "pvx_lookup_rows_grad")
-    return dtable, None, None, None
-
-
-_lookup_grad_once = once_differentiable(_lookup_grad)      # under create_graph: a second derivative is refused, not left out
+    return dtable
 
 
 def lookup_rows(table, index, scale=1.0, sort=None):
     """scale * table[index]: table [m, ...] float32 / float16 / bfloat16, index int32 or int64 of any shape -> [*index.shape, ...] in the
     table's dtype.  Entries outside [0, m) give zeros and pass no gradient.  The gradient with respect to the table (and only to it) adds
-    each row's entries in 32 bits and in an order of its own, without atomics.  `sort`: sort_index(index, m) of this very index, where the caller
-    has it (the backward sorts otherwise)."""
+    each row's entries in 32 bits and in an order of its own, without atomics, and can be differentiated again.  `sort`: sort_index(index, m)
+    of this very index, where the caller has it (the backward sorts otherwise)."""
     if not table.is_cuda:
         raise RuntimeError("rows are looked up on the GPU only (no CPU fallback): got a table on %s" % table.device)
     _check_index(index)

@@ -198,3 +198,32 @@ def test_voxel_encoders_take_the_lookup(cuda_device, monkeypatch):
         - torch.tensor([0.0, 0.0, 8.0, 2.0, 0.0], device=cuda_device)
     enc({"points": pts, "batch_size": 1})                                  # a fifth of the points lies outside
     assert len(calls) == 1 and calls[0] >= 0
+
+
+def test_lookup_differentiates_again(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    for n, m in ((300, 40), (20000, 700)):
+        table = torch.randn(m, 24, device=cuda_device, generator=g).requires_grad_(True)
+        index = torch.randint(-3, m + 3, (n,), device=cuda_device, generator=g)
+        v = torch.randn(m, 24, device=cuda_device, generator=g)
+        for sort in (None, scatter.sort_index(index, m)):
+            out = scatter.lookup_rows(table, index, scale=0.5, sort=sort)
+            first, = torch.autograd.grad((out ** 3).sum(), table, create_graph=True)
+            second, = torch.autograd.grad((first * v).sum(), table)
+            # L = sum (s T)^3 over the entries inside: dL = 3 s^3 T^2, times v, again: 6 s^3 T v, once an entry
+            count = torch.bincount(index[(index >= 0) & (index < m)], minlength=m).double().unsqueeze(1)
+            t64 = table.detach().double()
+            want = count * 6 * 0.125 * t64 * v.double()
+            assert torch.allclose(first.detach().double(), count * 3 * 0.125 * t64 ** 2, rtol=0, atol=float(count.max()) * 40 * U * float((t64 ** 2).max()))
+            assert bool(((second.double() - want).abs() <= (count + 12) * U * want.abs()).all())
+
+
+def test_voxel_encoder_layer_differentiates_again(cuda_device):
+    layer, x, inv, plain = _encoder_layer(cuda_device)
+    results = []
+    for f in (lambda a: layer(a, inv, 500), plain):
+        a = x.clone().requires_grad_(True)
+        first, = torch.autograd.grad((f(a) ** 2).sum(), a, create_graph=True)
+        results.append((first.detach(),) + torch.autograd.grad((first ** 2).sum(), [a, layer.linear.weight]))
+    for got, want in zip(*results):
+        assert float((got - want).norm()) <= 1e-5 * float(want.norm())        # sums of some 20 terms, in another order
