@@ -12,7 +12,7 @@ import torch
 from . import _lib
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # a s + b s^3 + c s^5: steepest at 0 of those that keep (0, 1] within about 0.7 .. 1.2
-MAX_MATRICES, MAX_STEPS = 64, 64              # of one call of the C entry
+MAX_MATRICES, MAX_STEPS, MAX_SIDE = 64, 64, 2 ** 20      # of one call of the C entry
 
 
 def _launch(mats, outs, steps, coefficients, eps):
@@ -37,6 +37,17 @@ def _launch(mats, outs, steps, coefficients, eps):
 def _check_coefficients(steps, coefficients):
     if not _lib.lib().pvx_orthogonalize_holds(steps, *coefficients):
         raise ValueError("%d steps of the coefficients %r do not keep the singular values within known bounds" % (steps, tuple(coefficients)))
+
+
+def _check_options(o):
+    """of a parameter group of Muon"""
+    if not o["lr"] >= 0.0 or not 0.0 <= o["momentum"] < 1.0 or not o["weight_decay"] >= 0.0:
+        raise ValueError("lr and weight_decay must not be negative and momentum must be in [0, 1): got %r, %r, %r"
+                         % (o["lr"], o["weight_decay"], o["momentum"]))
+    if not 0 <= o["steps"] <= MAX_STEPS or not o["eps"] >= 0.0 or len(o["coefficients"]) != 3:
+        raise ValueError("steps must be 0 .. %d and eps not negative, with three coefficients: got %r, %r, %r"
+                         % (MAX_STEPS, o["steps"], o["eps"], o["coefficients"]))
+    _check_coefficients(int(o["steps"]), o["coefficients"])
 
 
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -88,20 +99,41 @@ class Muon(torch.optim.Optimizer):
     [shape[0], everything else].  All matrices of a step are orthogonalised together."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
-        if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
-            raise ValueError("lr and weight_decay must not be negative and momentum must be in [0, 1): got %r, %r, %r" % (lr, weight_decay, momentum))
-        if not 0 <= int(steps) <= MAX_STEPS or not eps >= 0.0 or len(coefficients) != 3:
-            raise ValueError("steps must be 0 .. %d and eps not negative, with three coefficients: got %r, %r, %r" % (MAX_STEPS, steps, eps, coefficients))
-        _check_coefficients(int(steps), coefficients)
-        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps),
-                                      coefficients=tuple(coefficients), eps=eps))
+        defaults = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps), coefficients=tuple(coefficients),
+                        eps=eps)
+        _check_options(defaults)
+        super().__init__(params, defaults)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                self.param_groups.pop()
-                raise ValueError("Muon takes parameters of two and more dimensions, got %s: give the others to another optimiser" % (tuple(p.shape),))
+        try:
+            _check_options(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                if p.dim() < 2:
+                    raise ValueError("Muon takes parameters of two and more dimensions, got %s: give the others to another optimiser"
+                                     % (tuple(p.shape),))
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _groups_with_gradients(self):
+        """(group, its parameters that have a gradient) of every group, all of them looked at before any state changes"""
+        groups = []
+        for group in self.param_groups:
+            _check_options(group)
+            params = [p for p in group["params"] if p.grad is not None and p.numel() > 0]
+            for p in params:
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
+                if max(p.shape[0], p.numel() // p.shape[0]) > MAX_SIDE:
+                    raise ValueError("matrices have at most %d rows and columns, got a parameter %s" % (MAX_SIDE, tuple(p.shape)))
+                if not p.is_cuda:
+                    raise RuntimeError("orthogonalize runs on the GPU only (no CPU fallback): got a matrix on %s" % p.device)
+                if p.dtype not in _lib.DTYPE_CODE:
+                    raise TypeError("unsupported dtype %s" % p.dtype)
+            if params:
+                groups.append((group, params))
+        return groups
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -109,17 +141,7 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None and p.numel() > 0]
-            if not params:
-                continue
-            for p in params:
-                if p.grad.is_sparse:
-                    raise RuntimeError("Muon does not take sparse gradients")
-                if not p.is_cuda:                                        # refused before any state changes
-                    raise RuntimeError("orthogonalize runs on the GPU only (no CPU fallback): got a matrix on %s" % p.device)
-                if p.dtype not in _lib.DTYPE_CODE:
-                    raise TypeError("unsupported dtype %s" % p.dtype)
+        for group, params in self._groups_with_gradients():
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
                     self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)

@@ -227,3 +227,33 @@ def test_voxel_encoder_layer_differentiates_again(cuda_device):
         results.append((first.detach(),) + torch.autograd.grad((first ** 2).sum(), [a, layer.linear.weight]))
     for got, want in zip(*results):
         assert float((got - want).norm()) <= 1e-5 * float(want.norm())        # sums of some 20 terms, in another order
+
+
+# ---- the optimiser ---------------------------------------------------------------------------------------------------------
+def test_muon_refuses_in_any_group_before_it_changes_anything(cuda_device):
+    def setup(bad_shape=(4, 4), dtype=torch.float32, device=cuda_device):
+        good, bad = torch.nn.Parameter(torch.ones(4, 4, device=cuda_device)), torch.nn.Parameter(torch.ones(bad_shape, device=device, dtype=dtype))
+        good.grad, bad.grad = torch.ones_like(good), torch.ones_like(bad)
+        return good, bad, optim.Muon([dict(params=[good]), dict(params=[bad])])
+
+    def untouched(good, opt):
+        return float((good - 1).abs().max()) == 0 and not opt.state
+
+    for kw, error in ((dict(dtype=torch.float64), TypeError), (dict(device="cpu"), RuntimeError), (dict(bad_shape=(1, 2 ** 20 + 1)), ValueError),
+                      (dict(bad_shape=(2 ** 20 + 1, 1)), ValueError)):
+        good, bad, opt = setup(**kw)
+        with pytest.raises(error):
+            opt.step()
+        assert untouched(good, opt), kw
+    good, bad, opt = setup()
+    bad.grad = bad.grad.to_sparse()
+    with pytest.raises(RuntimeError):
+        opt.step()
+    assert untouched(good, opt)
+    for kw in (dict(steps=65), dict(steps=-1), dict(coefficients=(3.0, -2.0, 0.0)), dict(coefficients=(1.0, 2.0)), dict(eps=-1.0), dict(momentum=-3.0),
+               dict(momentum=1.0), dict(weight_decay=-1.0), dict(lr=-1.0), dict(lr=float("nan"))):
+        good, bad, opt = setup()
+        opt.param_groups[1].update(kw)                         # as a scheduler or a loaded state may
+        with pytest.raises(ValueError):
+            opt.step()
+        assert untouched(good, opt), kw

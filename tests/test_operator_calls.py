@@ -12,3 +12,28 @@ def test_counts_past_32_bits():
     for big in (2 ** 31, 2 ** 32 + 5):
         with pytest.raises(ValueError, match="op: a count of %d is past 32 bits" % big):
             _lib.check_counts("op", 3, big, 1)
+
+
+# ---- the optimiser's options -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(steps=100), dict(steps=-1), dict(coefficients=(3.0, -2.0, 0.0)), dict(coefficients=(1.0, 2.0)), dict(eps=-1.0),
+                                dict(eps=float("nan")), dict(momentum=-3.0), dict(momentum=1.0), dict(weight_decay=-1.0), dict(lr=-1.0)])
+def test_muon_refuses_options_of_a_group(kw):
+    w, v = (torch.nn.Parameter(torch.zeros(4, 4)) for _ in range(2))
+    with pytest.raises(ValueError):
+        optim.Muon([dict(params=[w], **kw)])
+    with pytest.raises(ValueError):
+        optim.Muon([w], **kw)
+    opt = optim.Muon([w])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[v], **kw))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[v], lr=0.1, momentum=0.5))           # refused groups leave nothing behind
+    assert [g["momentum"] for g in opt.param_groups] == [0.95, 0.5]
+
+
+def test_muon_refuses_matrices_past_the_largest():
+    for shape in ((2 ** 20 + 1, 1), (1, 2 ** 20 + 1), (2, 2 ** 10, 2 ** 10 + 1)):
+        w = torch.nn.Parameter(torch.zeros(shape))
+        w.grad = torch.zeros(shape)
+        with pytest.raises(ValueError, match="1048576"):
+            optim.Muon([w]).step()
