@@ -96,7 +96,9 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 class Muon(torch.optim.Optimizer):
     """momentum buf <- momentum buf + grad; update = orthogonalize(grad + momentum buf, or buf without nesterov);
     p <- (1 - lr weight_decay) p - lr max(1, rows / cols)^0.5 update, for parameters of two and more dimensions taken as the matrix
-    [shape[0], everything else].  All matrices of a step are orthogonalised together."""
+    [shape[0], everything else].  All matrices of a group are orthogonalised together.  The
+    momentum is float32 whatever the parameter's type (in 8 bits a gradient below 2^-8 of it would be lost), and so is all that follows up
+    to the one rounding of the new parameter."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         defaults = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps), coefficients=tuple(coefficients),
@@ -135,6 +137,13 @@ class Muon(torch.optim.Optimizer):
                 groups.append((group, params))
         return groups
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)              # which gives every state its parameter's type
+        saved = [state_dict["state"].get(k, {}) for group in state_dict["param_groups"] for k in group["params"]]
+        for p, state in zip((p for group in self.param_groups for p in group["params"]), saved):
+            if "momentum_buffer" in state:
+                self.state[p]["momentum_buffer"] = state["momentum_buffer"].to(device=p.device, dtype=torch.float32)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -144,18 +153,22 @@ class Muon(torch.optim.Optimizer):
         for group, params in self._groups_with_gradients():
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
-                    self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-            grads = [p.grad for p in params]
+                    self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+            grads = [p.grad.float() for p in params]                         # (of float32: the gradient itself)
             bufs = [self.state[p]["momentum_buffer"] for p in params]
             torch._foreach_mul_(bufs, group["momentum"])
             torch._foreach_add_(bufs, grads)
             updates = torch._foreach_add(grads, bufs, alpha=group["momentum"]) if group["nesterov"] else bufs
             mats = orthogonalize([u.reshape(u.shape[0], -1) for u in updates], group["steps"], group["coefficients"], group["eps"])
+            wide = [p if p.dtype == torch.float32 else p.float() for p in params]
             if group["weight_decay"] != 0.0:
-                torch._foreach_mul_(params, 1.0 - group["lr"] * group["weight_decay"])
+                torch._foreach_mul_(wide, 1.0 - group["lr"] * group["weight_decay"])
             by_scale = {}
-            for p, o in zip(params, mats):
+            for p, o in zip(wide, mats):
                 by_scale.setdefault(max(1.0, o.shape[0] / o.shape[1]) ** 0.5, []).append((p, o.view(p.shape)))
             for scale, pairs in by_scale.items():
                 torch._foreach_add_([p for p, _ in pairs], [o for _, o in pairs], alpha=-group["lr"] * scale)
+            narrow = [(p, q) for p, q in zip(params, wide) if p is not q]
+            if narrow:
+                torch._foreach_copy_([p for p, _ in narrow], [q for _, q in narrow])
         return loss

@@ -257,3 +257,58 @@ def test_muon_refuses_in_any_group_before_it_changes_anything(cuda_device):
         with pytest.raises(ValueError):
             opt.step()
         assert untouched(good, opt), kw
+
+
+def reference(m, steps=5, eps=1e-7, coefficients=optim.COEFFICIENTS):
+    a, b, c = coefficients
+    x = m.double()
+    tall = x.shape[0] > x.shape[1]
+    x = (x.t() if tall else x).contiguous()
+    x = x / (x.square().sum().sqrt() + eps)
+    for _ in range(steps):
+        g = x @ x.t().contiguous()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.t() if tall else x
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 1.0), (torch.float16, 1.0), (torch.float16, 2.0 ** -22), (torch.float32, 1.0)])
+def test_muon_keeps_its_momentum_in_32_bits(cuda_device, dtype, size, nesterov):
+    """Against the recurrence in 64 bits on the same gradients (2^-22: a few steps above the least of float16).  The momentum takes two
+    roundings a step of sums no larger than sum |grad|; a weight takes one of its type on (1 - lr decay) p - lr scale o, where o is within
+    3800 2^-24 of its own norm (the five steps of the polynomial on the halves of its operands) and four roundings of 32 bits come to it."""
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    lr, decay, mom = 0.05, 0.1, 0.9
+    shapes = [(16, 3, 3, 3, 5), (90, 16), (4, 4)]
+    params = [torch.nn.Parameter(torch.randn(s, device=cuda_device, generator=g).to(dtype)) for s in shapes]
+    opt = optim.Muon(params, lr=lr, momentum=mom, nesterov=nesterov, weight_decay=decay)
+    bufs = [torch.zeros(s, dtype=torch.float64, device=cuda_device) for s in shapes]
+    mags = [torch.zeros_like(b) for b in bufs]
+    for step in range(6):
+        before = [p.detach().double().clone() for p in params]
+        want = []
+        for k, p in enumerate(params):
+            p.grad = (torch.randn(p.shape, device=cuda_device, generator=g) * size + (size if step < 3 else 0.0)).to(dtype)
+            bufs[k] = mom * bufs[k] + p.grad.double()
+            mags[k] = mom * mags[k] + p.grad.double().abs()
+            u = p.grad.double() + mom * bufs[k] if nesterov else bufs[k]
+            o = reference(u.view(u.shape[0], -1))
+            scale = max(1.0, o.shape[0] / o.shape[1]) ** 0.5
+            want.append((before[k] * (1 - lr * decay) - lr * scale * o.view(u.shape), lr * scale * float(o.norm())))
+        opt.step()
+        for p, buf, mag, q, (w, o) in zip(params, bufs, mags, before, want):
+            got = opt.state[p]["momentum_buffer"]
+            assert got.dtype == torch.float32
+            assert bool(((got.double() - buf).abs() <= 2 * (step + 1) * U * mag).all())
+            tol = 3800 * U * o + 4 * U * (q.abs() + o)
+            tol = tol + torch.finfo(dtype).eps / 2 * (w.abs() + tol)
+            assert bool(((p.detach().double() - w).abs() <= tol).all()), "step %d, %s" % (step, tuple(p.shape))
+    again = optim.Muon([torch.nn.Parameter(p.detach().clone()) for p in params], lr=lr, momentum=mom, nesterov=nesterov, weight_decay=decay)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for p, q in zip(params, again.param_groups[0]["params"]):
+        assert torch.equal(opt.state[p]["momentum_buffer"], again.state[q]["momentum_buffer"])      # the type and the bits survive loading
+        p.grad = torch.randn(p.shape, device=cuda_device, generator=g).to(dtype)
+        q.grad = p.grad.clone()
+    opt.step()
+    again.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, again.param_groups[0]["params"]))
