@@ -70,7 +70,7 @@ class SparseSequential(SparseModule):
             module = mods[i]
             if is_spconv_module(module):
                 assert isinstance(input, SparseConvTensor)
-                act = norm.act_name(mods[i + 1]) if isinstance(module, norm.SparseGroupNorm) and i + 1 < len(mods) else None
+                act = norm.act_name(mods[i + 1]) if norm.takes_act(module) and i + 1 < len(mods) else None
                 if act is not None:     # the activation behind a group norm runs in its kernels
                     input = module(input, act=act)
                     i += 1

@@ -174,9 +174,15 @@ def bn_act(x, bn, residual=None, relu=True):
 _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
+def _hooked(module):
+    m = torch.nn.modules.module
+    return (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks or m._global_forward_hooks
+            or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks)
+
+
 def act_name(module):
-    """the name `group_norm_act` has for an activation module, None if it has none or the module has hooks that want its own call"""
-    if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+    """the name `group_norm_act` has for an activation module, None if it has none or hooks want the module's own call"""
+    if _hooked(module):
         return None
     if type(module) is nn.ReLU:
         return "relu"
@@ -357,8 +363,17 @@ class SparseGroupNorm(SparseModule):
                                                     offsets, order))
 
 
+def takes_act(module):
+    """whether a module is a group norm whose kernels may run what follows it: one with hooks, or a subclass, is called for the norm alone"""
+    return type(module) is SparseGroupNorm and not _hooked(module)
+
+
 def norm_act(x, norm, residual=None, relu=True):
     """relu?(norm(x) (+ residual)) for a SparseConvTensor x and a norm of either kind -> SparseConvTensor"""
-    if isinstance(norm, SparseGroupNorm):
+    if takes_act(norm):
         return norm(x, act="relu" if relu else None, residual=residual)
+    if isinstance(norm, SparseGroupNorm):
+        out = norm(x)
+        y = out.features if residual is None else out.features + residual.to(out.features.dtype)
+        return out.replace_feature(torch.relu(y) if relu else y)
     return x.replace_feature(bn_act(x.features, norm, residual=residual, relu=relu))

@@ -312,3 +312,46 @@ def test_muon_keeps_its_momentum_in_32_bits(cuda_device, dtype, size, nesterov):
     opt.step()
     again.step()
     assert all(torch.equal(p, q) for p, q in zip(params, again.param_groups[0]["params"]))
+
+
+class OldNorm(spconv.SparseGroupNorm):
+    def forward(self, input):                                  # the signature of any sparse module
+        return super().forward(input)
+
+
+def test_hooks_of_a_group_norm_see_the_norm(cuda_device):
+    feats, idx = _sites(cuda_device, 16)
+    make = lambda: spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)  # noqa: E731
+    gn = spconv.SparseGroupNorm(4, 16).to(cuda_device)
+    seq = spconv.SparseSequential(gn, torch.nn.ReLU())
+    want, alone = seq(make()).features, gn(make()).features
+    seen = []
+    handle = gn.register_forward_hook(lambda m, i, o: seen.append(o.features))
+    got = seq(make()).features
+    assert len(seen) == 1 and torch.equal(seen[0], alone) and torch.equal(got, want)      # the clamp of the same fp32 values
+    handle.remove()
+    assert torch.equal(spconv.SparseSequential(OldNorm(4, 16).to(cuda_device), torch.nn.ReLU())(make()).features, want)
+    called = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, i, o: called.append(type(m).__name__))
+    try:
+        assert torch.equal(seq(make()).features, want)
+    finally:
+        handle.remove()
+    assert called == ["SparseGroupNorm", "ReLU", "SparseSequential"]
+
+
+def test_hooks_of_a_residual_block_see_the_norm(cuda_device):
+    feats, idx = _sites(cuda_device, 16)
+    make = lambda: spconv.SparseConvTensor(feats, idx, [8, 20, 20], 3)  # noqa: E731
+    torch.manual_seed(0)
+    block = backbones.SparseBasicBlock(16, 16, norm_fn=lambda c: spconv.SparseGroupNorm(4, c), indice_key="k").to(cuda_device)
+    want = block(make()).features
+    seen = []
+    handles = [m.register_forward_hook(lambda m, i, o: seen.append(o.features)) for m in (block.bn1, block.bn2)]
+    got = block(make()).features
+    [h.remove() for h in handles]
+    assert len(seen) == 2 and all(float(s.min()) < 0 for s in seen)
+    assert torch.equal(got, want)                              # fp32: norm, + residual and clamp round as the fused form does
+    old = backbones.SparseBasicBlock(16, 16, norm_fn=lambda c: OldNorm(4, c), indice_key="k").to(cuda_device)
+    old.load_state_dict(block.state_dict())
+    assert torch.equal(old(make()).features, want)
