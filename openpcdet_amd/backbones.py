@@ -24,10 +24,21 @@ from .spconv import pytorch as spconv
 BN_EPS, BN_MOMENTUM = 1e-3, 0.01     # spconv_backbone.py:75,192
 
 
+def _norm_groups(model_cfg):
+    get = getattr(model_cfg, 'get', None)
+    return get('NORM_GROUPS', None) if get is not None else getattr(model_cfg, 'NORM_GROUPS', None)
+
+
+def batch_norm_only(model_cfg, name):
+    """for models without the choice of `_norm`: a config that asks for it must not get BatchNorm without a word"""
+    if _norm_groups(model_cfg):
+        raise ValueError("%s has batch norm only: NORM_GROUPS is for VoxelBackBone8x, VoxelResBackBone8x and VoxelResBackBone8xVoxelNeXt" % name)
+
+
 def _norm(model_cfg=None):
     """BatchNorm1d as the reference has it, or, with NORM_GROUPS in the model config, a group norm of that many groups per frame (no
     statistics over the batch, nothing to synchronise between ranks)"""
-    groups = model_cfg.get('NORM_GROUPS', None) if model_cfg is not None and hasattr(model_cfg, 'get') else None
+    groups = _norm_groups(model_cfg)
     if groups:
         return partial(spconv.SparseGroupNorm, int(groups))
     return partial(nn.BatchNorm1d, eps=BN_EPS, momentum=BN_MOMENTUM)
@@ -244,7 +255,7 @@ class VoxelResBackBone8xVoxelNeXt(nn.Module):
             norm_fn(out_channel), nn.ReLU())
         self.shared_conv = spconv.SparseSequential(
             spconv.SubMConv2d(out_channel, out_channel, 3, stride=1, padding=1, bias=True),
-            norm_fn(out_channel) if get('NORM_GROUPS', None) else nn.BatchNorm1d(out_channel), nn.ReLU(True))
+            norm_fn(out_channel) if _norm_groups(model_cfg) else nn.BatchNorm1d(out_channel), nn.ReLU(True))
         self.forward_ret_dict = {}
         self.num_point_features = out_channel
         self.backbone_channels = {'x_conv1': ch[0], 'x_conv2': ch[1], 'x_conv3': ch[2], 'x_conv4': ch[3]}

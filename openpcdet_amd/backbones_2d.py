@@ -12,6 +12,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from .backbones import batch_norm_only
 from .spconv import pytorch as spconv
 
 
@@ -79,6 +80,7 @@ class _PillarBackbone(nn.Module):
 
     def __init__(self, model_cfg=None, input_channels=None, grid_size=None, **kwargs):
         super().__init__()
+        batch_norm_only(model_cfg, type(self).__name__)
         self.model_cfg = model_cfg
         grid_size = np.asarray(grid_size)
         self.sparse_shape = grid_size[[1, 0]]                                   # (H, W) = (ny, nx)
@@ -130,6 +132,7 @@ class VoxelResBackBone8xVoxelNeXt2D(nn.Module):
 
     def __init__(self, model_cfg=None, input_channels=None, grid_size=None, **kwargs):
         super().__init__()
+        batch_norm_only(model_cfg, type(self).__name__)
         self.model_cfg = model_cfg
         bn1 = partial(nn.BatchNorm1d, eps=1e-3, momentum=0.01)
         self.sparse_shape = np.asarray(grid_size)[[1, 0]]

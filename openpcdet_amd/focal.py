@@ -21,7 +21,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from .backbones import SparseBasicBlock, post_act_block  # noqa: F401  (re-exported like spconv_backbone_focal.py:40-98)
+from .backbones import SparseBasicBlock, batch_norm_only, post_act_block  # noqa: F401  (re-exported like spconv_backbone_focal.py:40-98)
 from .spconv import pytorch as spconv
 
 
@@ -225,6 +225,7 @@ class VoxelBackBone8xFocal(nn.Module):
 
     def __init__(self, model_cfg, input_channels, grid_size, **kwargs):
         super().__init__()
+        batch_norm_only(model_cfg, type(self).__name__)
         self.model_cfg = model_cfg
         cfg = model_cfg if model_cfg is not None else {}
         norm_fn = partial(nn.BatchNorm1d, eps=1e-3, momentum=0.01)

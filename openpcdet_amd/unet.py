@@ -9,13 +9,14 @@ import numpy as np
 import torch
 from torch import nn
 
-from .backbones import SparseBasicBlock, post_act_block
+from .backbones import SparseBasicBlock, batch_norm_only, post_act_block
 from .spconv import pytorch as spconv
 
 
 class UNetV2(nn.Module):
     def __init__(self, model_cfg=None, input_channels=None, grid_size=None, voxel_size=None, point_cloud_range=None, **kwargs):
         super().__init__()
+        batch_norm_only(model_cfg, type(self).__name__)
         self.model_cfg = model_cfg
         cfg = model_cfg if model_cfg is not None else {}
         self.sparse_shape = [int(v) for v in (np.asarray(grid_size)[::-1] + [1, 0, 0])]

@@ -37,3 +37,12 @@ def test_muon_refuses_matrices_past_the_largest():
         w.grad = torch.zeros(shape)
         with pytest.raises(ValueError, match="1048576"):
             optim.Muon([w]).step()
+
+
+# ---- NORM_GROUPS -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("make", [unet.UNetV2, focal.VoxelBackBone8xFocal, backbones_2d.PillarBackBone8x, backbones_2d.PillarRes18BackBone8x,
+                                  backbones_2d.VoxelResBackBone8xVoxelNeXt2D])
+def test_models_without_group_norm_say_so(make):
+    """the key is of the voxel backbones: a model that has BatchNorm only must not take it for nothing"""
+    with pytest.raises(ValueError, match="NORM_GROUPS"):
+        make(model_cfg={"NORM_GROUPS": 4}, input_channels=5, grid_size=[64, 64, 40])
