@@ -643,8 +643,11 @@ bool all_small(const pvx_matrix* mats, int count) {
 
 int round_up(int v, int to) { return PVX_CDIV(v, to) * to; }
 
-// 128 x 128 tiles where the widest product fills the chip with them (they read LDS half as often), 64 x 64 otherwise (128 / 64:
-// 2048 x 4096 1167 / 1422 us, 2048 x 2048 782 / 884, 1024 x 1024 342 / 257, 512 x 2304 245 / 190)
+// 128 x 128 tiles where the products of all matrices of the call together fill the chip with them (they read LDS half as often), 64 x 64
+// otherwise (128 / 64: 2048 x 4096 1167 / 1422 us, 2048 x 2048 782 / 884, 1024 x 1024 342 / 257, 512 x 2304 245 / 190).  One tile for a
+// call: lists of wide matrices gain (64 of 256 x 2304 1188 / 1462, 8 of 1024 x 1024 887 / 1047, 8 of 512 x 2304 541 / 633, 2 of 1536 x 2048
+// 870 / 945), lists near the border stay within 6 % (16 of 256 x 2304 431 / 407, 5 of 1024 x 1024 668 / 656, 3 of 1024 x 2048 696 / 706), and
+// many narrow ones, padded to 128 rows, lose (42 layers of 16 to 128 rows 333 / 265).
 int tile_of(const pvx_matrix* mats, int count) {
     double tiles = 0.0;
     for (int i = 0; i < count; i++) tiles += (double)mats[i].rows * mats[i].cols / (128.0 * 128.0);
