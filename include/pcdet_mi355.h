@@ -585,6 +585,7 @@ int pvx_group_norm_act_bwd(const void* dy, const void* x, const void* residual, 
  * The products keep their operands against a bound of the singular values that is followed through the steps.  Coefficients for which
  * that bound says too little (from a start in [1/64, 1] it leaves a factor of 128 between the largest value's bounds, or passes 10^9)
  * are PVX_ERR_RANGE; pvx_orthogonalize_holds is 1 for those that are taken.
+ * (A start below 1/64, which takes a shorter side past 4096, is covered by the slope at 0 of what is taken.)
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct { const void* in; void* out; int rows, cols; } pvx_matrix;
 #define PVX_ORTHO_MAX 64

@@ -172,6 +172,10 @@ Poly poly_of(float a, float b, float c) {
 // its last step, so with r <= 128 lo an entry of A, kept against r^2, is off by at most 2^-25 of the square of the largest value: as
 // binary32.  3 x - 2 x^3 shows what must not pass: the values stay below sqrt(2), at whose end the slope is -9, but 1 % more makes the
 // bound 1.4, 1.6, 2.9, 39, 1e5, and everything is lost below f16's last step.  A norm near eps starts lower: 2^0, 2^-2, .. 2^-20.
+// More than 4096 rows may start lower still, at 1 / sqrt(rows), down to 2^-10, beside a bound of 1.  What is accepted here has its slope a to
+// within 1 % on [0, 1 / 64] (128 |f(1 / 64)| >= the largest |f| leaves |b| and |c| no more than some ten times |a|), so such a value goes
+// through a I alone until it reaches the range that was followed; A's words matter beside a, not beside the value, and only X's own are
+// nearer to f16's last step: off by up to 2^-28 of the largest value, at 2^20 rows, instead of 2^-32.
 bool bound_holds(int steps, float a, float b, float c) {
     constexpr double kSpread = 128.0, kMost = 1e9;       // kMost: where above() ends
     const Poly p = poly_of(a, b, c);

@@ -355,3 +355,22 @@ def test_hooks_of_a_residual_block_see_the_norm(cuda_device):
     old = backbones.SparseBasicBlock(16, 16, norm_fn=lambda c: OldNorm(4, c), indice_key="k").to(cuda_device)
     old.load_state_dict(block.state_dict())
     assert torch.equal(old(make()).features, want)
+
+
+# ---- orthogonalisation -----------------------------------------------------------------------------------------------------
+def test_many_equal_singular_values(cuda_device):
+    """16384 orthogonal rows: every singular value is 1 / 128 of the norm, and the result is a multiple of the matrix that the polynomial
+    on one number gives.  A step adds up to three roundings of 2.7 2^-24 and the sums' sqrt(6 k / 16), here over k = 16384 three times."""
+    h = torch.ones(1, 1, device=cuda_device)
+    while h.shape[0] < 16384:
+        h = torch.cat([torch.cat([h, h], 1), torch.cat([h, -h], 1)], 0)
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    h = h * (2.0 * torch.randint(0, 2, (16384,), device=cuda_device, generator=g) - 1)      # other signs for the columns
+    got = optim.orthogonalize(h)
+    a, b, c = optim.COEFFICIENTS
+    t = 1.0 / 128
+    for _ in range(5):
+        t = a * t + b * t ** 3 + c * t ** 5
+    want = t / 128                                             # the entries of h / |h| times the ratio of t to 1 / 128
+    err = (got.double() - want * h.double()).norm() / (want * 16384)
+    assert float(err) <= (40 + 5 * 3 * (6 * 16384 / 16) ** 0.5) * U

@@ -1,5 +1,7 @@
 """CPU: checks of the training-step operators' Python entries that need no GPU: counts past 32 bits, options of an optimiser's groups, models that
 take no group norm."""
+import random
+
 import pytest
 import torch
 
@@ -46,3 +48,16 @@ def test_models_without_group_norm_say_so(make):
     """the key is of the voxel backbones: a model that has BatchNorm only must not take it for nothing"""
     with pytest.raises(ValueError, match="NORM_GROUPS"):
         make(model_cfg={"NORM_GROUPS": 4}, input_channels=5, grid_size=[64, 64, 40])
+
+
+# ---- coefficients ----------------------------------------------------------------------------------------------------------
+def test_accepted_polynomials_are_their_slope_near_zero():
+    """the range that is followed starts at 1/64; below it, where more than 4096 equal singular values start, a + b y + c y^2 has to be a"""
+    r, taken = random.Random(1), 0
+    for _ in range(50000):
+        a = r.uniform(-4, 4)
+        b, c = a * r.uniform(-12, 12), a * r.uniform(-12, 12)
+        if _lib.lib().pvx_orthogonalize_holds(1, a, b, c):
+            taken += 1
+            assert max(abs(b * y + c * y * y) for y in (2.0 ** -12, 2.0 ** -13)) <= 0.01 * abs(a)
+    assert taken > 500
