@@ -374,3 +374,44 @@ def test_many_equal_singular_values(cuda_device):
     want = t / 128                                             # the entries of h / |h| times the ratio of t to 1 / 128
     err = (got.double() - want * h.double()).norm() / (want * 16384)
     assert float(err) <= (40 + 5 * 3 * (6 * 16384 / 16) ** 0.5) * U
+
+
+def test_lists_and_views_as_near_as_single_matrices(cuda_device):
+    """matrices at least twice as wide as high, so that no direction is amplified beyond the result itself: three roundings a step of up to
+    2.7 2^-24 each over five steps make 40, and the sums over k in steps of 16 add sqrt(6 k / 16) of one rounding each, one over n and two
+    over m a step"""
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    shapes = [(16, 135)] + [(16, 432)] * 4 + [(432, 16), (128, 384), (64, 864), (256, 2304), (300, 7)]
+    mats = [torch.randn(s, device=cuda_device, generator=g) for s in shapes]
+    base = torch.randn(60, 400, device=cuda_device, generator=g)
+    mats += [base[:, ::2], base[1::3], base.t(), base.t()[::2]]
+    batch = torch.randn(3, 20, 50, device=cuda_device, generator=g)
+    outs = list(optim.orthogonalize(mats)) + list(optim.orthogonalize(batch).unbind(0)) + list(optim.orthogonalize([m.bfloat16() for m in mats]))
+    for o, m in zip(outs, mats + list(batch.unbind(0)) + [m.bfloat16() for m in mats]):
+        want, k = reference(m), (min(m.shape), max(m.shape))
+        sums = 5 * ((6 * k[1] / 16) ** 0.5 + 2 * (6 * k[0] / 16) ** 0.5)
+        rel = float((o.double() - want).norm() / want.norm())
+        assert rel <= (40 + sums) * U + torch.finfo(m.dtype).eps / 2, (tuple(m.shape), rel)
+
+
+# ---- the longest list of a lookup ------------------------------------------------------------------------------------------
+def test_lookup_of_nearly_2_31_entries(cuda_device):
+    n, m = 2 ** 31 - 2 ** 20 - 1, 3
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    index = torch.randint(-1, m + 1, (n,), device=cuda_device, dtype=torch.int32, generator=g)
+    table = torch.tensor([[1.0], [2.0], [4.0]], device=cuda_device, requires_grad=True)
+    out = scatter.lookup_rows(table, index)
+    parts = [slice(k, min(n, k + 2 ** 27)) for k in range(0, n, 2 ** 27)]
+    values = torch.tensor([0.0, 1.0, 2.0, 4.0, 0.0], device=cuda_device)
+    assert all(torch.equal(out.detach()[p, 0], values[index[p].long() + 1]) for p in parts)
+    up = torch.empty(n, 1, device=cuda_device)
+    up.normal_(generator=g)
+    got, = torch.autograd.grad(out, table, up)
+    del out
+    for v in range(m):
+        total = size = count = 0.0
+        for p in parts:
+            d = up[p, 0].double() * (index[p] == v)
+            total, size, count = total + float(d.sum()), size + float(d.abs().sum()), count + float((index[p] == v).sum())
+        # blocks of 64 on four levels: 3 (64 - 1) blocks and as many additions within the ends, and the last level's count / 64^4
+        assert abs(float(got[v]) - total) <= (4 * 64 + 6 * 63 + count / 64 ** 4 + 2) * U * size
