@@ -11,7 +11,8 @@ import torch
 
 from . import _lib
 
-COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # a s + b s^3 + c s^5: steepest at 0 of those that keep (0, 1] within about 0.7 .. 1.2
+# a s + b s^3 + c s^5: steepest at 0 of those that keep (0, 1] within about 0.7 .. 1.2 (published with the Muon optimiser, K. Jordan et al., 2024)
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_MATRICES, MAX_STEPS, MAX_SIDE = 64, 64, 2 ** 20      # of one call of the C entry
 
 
@@ -56,7 +57,8 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
     matrices: a matrix [r, c], a batch of them [B, r, c], or a list or tuple of matrices of any sizes; float32 / float16 / bfloat16, on the
     GPU.  The result has the same form, in the inputs' dtypes; whatever they are, the products are as accurate as binary32's.  No gradient flows through it.
-    Matrices of one dtype go through the GPU together, up to 64 in a call.  Coefficients whose polynomial does not keep the singular values
+    Matrices of one dtype go through the GPU together, up to 64 in a call: the tiles and parts of its products, and so the last bits of a
+    result, depend on the list that a matrix is in; the same list gives the same bits.  Coefficients whose polynomial does not keep the singular values
     within known bounds over the steps (a root or a fixed point that repels inside [0, 1], or growth past 1e9) are refused."""
     one = isinstance(matrices, torch.Tensor)
     if one and matrices.dim() not in (2, 3):
@@ -96,9 +98,9 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 class Muon(torch.optim.Optimizer):
     """momentum buf <- momentum buf + grad; update = orthogonalize(grad + momentum buf, or buf without nesterov);
     p <- (1 - lr weight_decay) p - lr max(1, rows / cols)^0.5 update, for parameters of two and more dimensions taken as the matrix
-    [shape[0], everything else].  All matrices of a group are orthogonalised together.  The
-    momentum is float32 whatever the parameter's type (in 8 bits a gradient below 2^-8 of it would be lost), and so is all that follows up
-    to the one rounding of the new parameter."""
+    [shape[0], everything else], of at most 2^20 rows and columns.  All matrices of a group are orthogonalised together.  The momentum is
+    float32 whatever the parameter's type (in 8 bits a gradient below 2^-8 of it would be lost), and so is all that follows up to the one
+    rounding of the new parameter.  A step that is refused has changed nothing."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         defaults = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps), coefficients=tuple(coefficients),
