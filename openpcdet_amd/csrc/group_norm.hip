@@ -113,6 +113,9 @@ struct Rows {
         }
         return lo;
     }
+    // behind an empty sample s at position p: the one before the next that has p, so that a run of empty ones costs a search and not a step
+    // each (700 rows in the first and last of 2^20 samples: forward 0.07 ms, 555 one by one)
+    __device__ __forceinline__ int skip(int s, int p) const { return max(s, first(p) - 1); }
     // row at position p (kept inside the matrix, whatever `order` holds)
     __device__ __forceinline__ int row(int p) const { return order ? (int)min((unsigned)order[p], (unsigned)(n - 1)) : p; }
 };
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_sums_kernel(const E* __res
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), lo = max(p0, begin), hi = min(p1, rows.begin(s + 1));
         if (begin >= p1) break;
-        if (lo >= hi) continue;
+        if (lo >= hi) { s = rows.skip(s, lo); continue; }
         double s0[V], s1[V];
 #pragma unroll
         for (int j = 0; j < V; j++) { s0[j] = 0; s1[j] = 0; }
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_apply_kernel(const E* __re
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), end = rows.begin(s + 1), lo = max(p0, begin), hi = min(p1, end);
         if (begin >= p1) break;
-        if (lo >= hi) continue;
+        if (lo >= hi) { s = rows.skip(s, lo); continue; }
         for (int p = done + t.r_in; p < lo && t.on; p += t.rpb) {       // positions of no sample
             const int row = rows.row(p);
             store_pack<E, V>(y + (size_t)row * c + t.chunk * V, zero);
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_sums_kernel(const E* _
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), lo = max(p0, begin), hi = min(p1, rows.begin(s + 1));
         if (begin >= p1) break;
-        if (lo >= hi) continue;
+        if (lo >= hi) { s = rows.skip(s, lo); continue; }
         double s0[V], s1[V];
         Chan<V> k;
 #pragma unroll
@@ -560,7 +563,7 @@ __global__ __launch_bounds__(kBlk, kResident) void gn_bwd_apply_kernel(const E* 
     for (int s = rows.first(p0); s < rows.samples; s++) {
         const int begin = rows.begin(s), end = rows.begin(s + 1), lo = max(p0, begin), hi = min(p1, end);
         if (begin >= p1) break;
-        if (lo >= hi) continue;
+        if (lo >= hi) { s = rows.skip(s, lo); continue; }
         for (int p = done + t.r_in; p < lo && t.on; p += t.rpb) {
             const int row = rows.row(p);
             const size_t off = (size_t)row * c + t.chunk * V;

@@ -415,3 +415,31 @@ def test_lookup_of_nearly_2_31_entries(cuda_device):
             total, size, count = total + float(d.sum()), size + float(d.abs().sum()), count + float((index[p] == v).sum())
         # blocks of 64 on four levels: 3 (64 - 1) blocks and as many additions within the ends, and the last level's count / 64^4
         assert abs(float(got[v]) - total) <= (4 * 64 + 6 * 63 + count / 64 ** 4 + 2) * U * size
+
+
+# ---- runs of empty samples -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("samples", [60, 1000, 2 ** 25])
+def test_norm_with_runs_of_empty_samples(cuda_device, samples):
+    """as without them; in no more time than the search takes (a step for each of 2^25 would be 18 s a pass)"""
+    n = 9000
+    rows = torch.zeros(samples, dtype=torch.int32, device=cuda_device)
+    rows[[0, samples // 3, samples // 3 + 1, samples - 2]] = torch.tensor([1200, 1, 3799, 4000], dtype=torch.int32, device=cuda_device)
+    off = torch.cat([rows.new_zeros(1), rows.cumsum(0, dtype=torch.int32)])
+    x = torch.randn(n, 16, device=cuda_device)
+    up = torch.randn(n, 16, device=cuda_device)
+    w = torch.rand(16, device=cuda_device) + 0.5
+    results = []
+    for o in (off, torch.unique(off).int()):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        y = norm.group_norm_act(leaves[0], 4, leaves[1], act="silu", offsets=o)
+        torch.cuda.synchronize()
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        y = norm.group_norm_act(leaves[0], 4, leaves[1], act="silu", offsets=o)
+        grads = torch.autograd.grad(y, leaves, up)
+        end.record()
+        end.synchronize()
+        results.append((y.detach(),) + grads)
+        assert start.elapsed_time(end) < 5000
+    for got, want in zip(*results):
+        assert float((got - want).abs().max()) <= 64 * U * float(want.abs().max())      # the same pieces, summed in another order in 64 bits
